@@ -376,6 +376,66 @@ VB_API int vb_nll_row_grad(void *logits, int64_t stride, const int64_t *targets,
                            const float *log_total, const float *grad, int64_t rows, int V,
                            int dtype, void *stream);
 
+/* ---- rows in 8 bits -------------------------------------------------------------------------
+ * Codes in [-127, 127] with one float32 scale per row, value = code * scale: scale = max|y| / 127,
+ * code = rint(y * 127 / max|y|). A row of magnitude below 1e-35 has scale 0 and codes 0; a row that
+ * holds a value that is not finite has scale NaN and codes 0 (it stands for NaN everywhere).
+ * q: int8 rows `ldq` bytes apart (ldq >= width; the bytes between width and ldq are not written).
+ *
+ * vb_rms_norm_q8: y is the RMSNorm of x (vb_rms_norm_fwd's arithmetic, vesper/column.py:159-188), or,
+ * with r, of sum = x + r (x, sum float32; r float32, bf16 or f16, r and sum both given or both NULL).
+ * vb_quantize_rows_q8: y is x (rows `ldx` elements apart) or, with relu_square, relu(x)^2 formed in
+ * float32 (vesper/ffn.py:44-56). vb_dequantize_rows_q8: the values, [rows, width] of `dtype`. */
+VB_API int vb_rms_norm_q8(const void *x, const void *r, const float *weight, float *sum, int8_t *q,
+                          int64_t ldq, float *scale, int64_t rows, int width, float floor_,
+                          float eps, int x_dtype, int r_dtype, void *stream);
+VB_API int vb_quantize_rows_q8(const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale,
+                               int64_t rows, int width, int relu_square, int dtype, void *stream);
+VB_API int vb_dequantize_rows_q8(const int8_t *q, int64_t ldq, const float *scale, void *y,
+                                 int64_t rows, int width, int dtype, void *stream);
+
+/* The quantised linear layer: y [M, N] of `dtype` (dense) = (sum_k xq[m,k] wq[n,k]) xs[m] ws[n], the
+ * sum exact in int32 (K <= 131056), scaled in float32 and rounded once. xq [M, K] and wq [N, K] int8,
+ * rows ldx and ldw bytes apart, 16-byte aligned, ldx and ldw multiples of 16; xs [M], ws [N] float32.
+ * `status`: an int32 on the device into which a kernel ORs 1 if a bounded wait gave up. Takes the
+ * place of the F.linear of vesper/column.py:236-253 and vesper/ffn.py:44-56 in quantised decoding. */
+VB_API int vb_linear_q8(const int8_t *xq, int64_t ldx, const float *xs, const int8_t *wq,
+                        int64_t ldw, const float *ws, void *y, int M, int N, int K, int dtype,
+                        int *status, void *stream);
+
+/* ---- a ring cache held in 4 bits ----------------------------------------------------------
+ * A RingKVCache (vesper/attention.py:63-139) of W positions whose keys and values take 4 bits a
+ * channel and two bf16 numbers a group of GS channels (32 where DK is a multiple of 32, else 16):
+ * lo = min rounded down, step = (max - lo) / 15 rounded up, code = rint((x - lo) / step), value =
+ * lo + code * step. k_codes, v_codes: [B, HKV, SLOTS, DK / 2] bytes, 16-byte aligned; k_params,
+ * v_params: [B, HKV, SLOTS, DK / GS, 2] bf16 (step, lo), 16-byte aligned; ring_pos [B, SLOTS] int64,
+ * -1 where nothing was written. SLOTS is W rounded up to a multiple of 64, DK a multiple of 16 up to
+ * 128; a token at position p lives in slot p % W. The order of the channels in a slot's bytes:
+ * csrc/q4.cuh. `dtype` is the element type of k, v, q and o.
+ *
+ * vb_q4_write: tokens k, v [B, N, HKV, DK] (batch and token strides in elements) at pos [B, N] int64,
+ * consecutive along a row; a negative position (padding) is not written, and of tokens that share a
+ * slot (N > W) the last is kept. vb_q4_read: the values held at pos [B, N], zeros and held = 0 where
+ * the ring does not hold that position. vb_q4_attend: one token per row, q [B, H, DK], k_new, v_new
+ * [B, HKV, DK] (row strides in elements), pos [B]: the token is written and attends the slots with
+ * p - W < pos <= p, itself included, as the ring holds them (scale 1/sqrt(DK), head h reading key
+ * head h / (H / HKV)); o [B, H, DK], zero in a row whose position is negative (which writes nothing).
+ * `workspace`: vb_q4_attend_workspace bytes. */
+VB_API int vb_q4_write(void *k_codes, void *k_params, void *v_codes, void *v_params,
+                       int64_t *ring_pos, const void *k, int64_t k_batch, int64_t k_token,
+                       const void *v, int64_t v_batch, int64_t v_token, const int64_t *pos, int B,
+                       int N, int HKV, int DK, int W, int SLOTS, int dtype, void *stream);
+VB_API int vb_q4_read(const void *k_codes, const void *k_params, const void *v_codes,
+                      const void *v_params, const int64_t *ring_pos, const int64_t *pos, void *k,
+                      void *v, uint8_t *held, int B, int N, int HKV, int DK, int W, int SLOTS,
+                      int dtype, void *stream);
+VB_API size_t vb_q4_attend_workspace(int B, int H, int HKV, int DK, int W);
+VB_API int vb_q4_attend(const void *q, int64_t q_row, const void *k_new, int64_t k_row,
+                        const void *v_new, int64_t v_row, const int64_t *pos, void *k_codes,
+                        void *k_params, void *v_codes, void *v_params, int64_t *ring_pos, void *o,
+                        void *workspace, int B, int H, int HKV, int DK, int W, int SLOTS, int dtype,
+                        void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -73,6 +73,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vb_relu_square_fwd": (_I, [_P, _P, ctypes.c_longlong, _I, _P]),
     "vb_relu_square_bwd": (_I, [_P, _P, _P, ctypes.c_longlong, _I, _P]),
     "vb_rotary": (_I, [_P, _P, _P, _P, ctypes.c_longlong, _I, _I, _I, _I, _P]),
+    "vb_rms_norm_q8": (_I, [_P] * 5 + [_I64, _P, _I64, _I, _F, _F, _I, _I, _P]),
+    "vb_quantize_rows_q8": (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P]),
+    "vb_dequantize_rows_q8": (_I, [_P, _I64, _P, _P, _I64, _I, _I, _P]),
+    "vb_linear_q8": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "vb_q4_write": (_I, [_P] * 6 + [_I64, _I64, _P, _I64, _I64, _P] + [_I] * 7 + [_P]),
+    "vb_q4_read": (_I, [_P] * 9 + [_I] * 7 + [_P]),
+    "vb_q4_attend_workspace": (_SZ, [_I, _I, _I, _I, _I]),
+    "vb_q4_attend": (_I, [_P, _I64, _P, _I64, _P, _I64] + [_P] * 8 + [_I] * 7 + [_P]),
     "vb_residual_add": (_I, [_P, _P, _P, _P, ctypes.c_longlong, _I, _I, _P]),
     "vb_residual_add_bwd": (_I, [_P, _P, _P, _P, ctypes.c_longlong, _I, _I, _P]),
 }

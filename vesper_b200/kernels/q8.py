@@ -1,0 +1,226 @@
+"""Quantised linear layers on a B200: rows in 8 bits with a scale each, and the int8 product over them.
+
+PRIMITIVES for serving (no gradients), what a decode step runs in place of a norm followed by a
+bf16 ``F.linear`` (``vesper/column.py:159-188`` with ``:236-253``, ``vesper/ffn.py:44-56`` of
+mstampfli/vesper-preview):
+
+- ``rms_norm_q8(x, weight, floor, eps) -> (q, scale)``: the column's RMSNorm with its output in 8 bits;
+- ``add_rms_norm_q8(x, r, weight, floor, eps) -> (s, q, scale)``: the same of ``s = x + r`` over a
+  float32 residual stream, the sum stored too, one kernel;
+- ``quantize_rows_q8(x, relu_square=False) -> (q, scale)``: any rows, or their squared ReLU;
+- ``dequantize_rows_q8(q, scale, dtype)``: the values back;
+- ``linear_q8(xq, xs, wq, ws, out_dtype)``: ``(xq @ wq.T) * xs[:, None] * ws``, summed exactly in int32.
+
+A row ``y`` becomes codes ``rint(y * 127 / max|y|)`` in ``[-127, 127]`` and ``scale = max|y| / 127``
+(float32). A row of magnitude below 1e-35 has scale 0; one that holds an infinity or a NaN has
+codes 0 and a NaN scale, so whatever is made from it is NaN, as it would be without the codes.
+A weight matrix is quantised once, by rows (output channels), with ``quantize_rows_q8``.
+
+The code tensors are ``[..., W]`` with rows padded to a multiple of 16 bytes (the product's copies
+start on 16-byte boundaries); ``linear_q8`` copies operands that are not laid out so.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from vesper_b200 import _lib
+from vesper_b200.contracts import ContractError, Dims, check_shape, require_cuda
+
+SUPPORTED = (torch.float32, torch.bfloat16, torch.float16)
+MAX_K = 131056  # largest inner dimension whose int8 sums stay in int32
+
+
+def serving_only(what: str, *tensors: Tensor | None) -> None:
+    """Refuse inputs that autograd is recording: these operators have no gradient."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        msg = f"the {what} has no gradient: call it under torch.no_grad()"
+        raise ContractError(msg)
+
+
+def _codes(x: Tensor) -> tuple[Tensor, Tensor, int]:
+    """Empty codes and scales for ``x``'s rows, and the codes' row pitch."""
+    width = x.shape[-1]
+    pitch = -(-width // 16) * 16
+    q = torch.empty(*x.shape[:-1], pitch, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    return (q if pitch == width else q[..., :width]), scale, pitch
+
+
+def _check_norm(x: Tensor, weight: Tensor, what: str) -> None:
+    require_cuda(what, x, weight=weight)
+    if x.dtype not in SUPPORTED:
+        msg = f"x: dtype must be one of {SUPPORTED}, got {x.dtype}"
+        raise ContractError(msg)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        msg = f"x: expected rows of at least one channel, got shape {tuple(x.shape)}"
+        raise ContractError(msg)
+    if weight.shape != (x.shape[-1],):
+        msg = f"weight: expected shape ({x.shape[-1]},), got {tuple(weight.shape)}"
+        raise ContractError(msg)
+
+
+def _norm(x: Tensor, r: Tensor | None, weight: Tensor, floor: float, eps: float):
+    serving_only("8-bit RMSNorm", x, r, weight)
+    width = x.shape[-1]
+    x = x.contiguous()
+    w32 = weight.to(torch.float32).contiguous()
+    q, scale, pitch = _codes(x)
+    total = None if r is None else torch.empty_like(x)
+    _lib.call(
+        "vb_rms_norm_q8", x.data_ptr(), _lib.ptr(r), w32.data_ptr(), _lib.ptr(total), q.data_ptr(), pitch,
+        scale.data_ptr(), x.numel() // width, width, floor, eps, _lib.DTYPE_CODE[x.dtype],
+        _lib.DTYPE_CODE[x.dtype if r is None else r.dtype], _lib.stream(x.device),
+    )  # fmt: skip
+    return total, q, scale
+
+
+def rms_norm_q8(x: Tensor, weight: Tensor, floor: float, eps: float) -> tuple[Tensor, Tensor]:
+    """``(q [..., W] int8, scale [...] float32)`` of ``fused_rms_norm(x, weight, floor, eps)``.
+
+    The norm is computed and quantised in float32 whatever ``x``'s dtype (float32, bf16 or f16).
+
+    Raises:
+        ContractError: on a CPU tensor, an unsupported dtype or a weight of another width.
+    """
+    _check_norm(x, weight, "8-bit RMSNorm")
+    _, q, scale = _norm(x, None, weight, floor, eps)
+    return q, scale
+
+
+def add_rms_norm_q8(x: Tensor, r: Tensor, weight: Tensor, floor: float, eps: float) -> tuple[Tensor, Tensor, Tensor]:
+    """``(s, q, scale)``: ``s = x + r`` (float32) and ``rms_norm_q8(s, weight, floor, eps)``, one kernel.
+
+    ``x`` is the float32 residual stream, ``r`` a sublayer's output of the same shape (float32, bf16
+    or f16); the sum is one IEEE float32 addition per channel, as torch's mixed-dtype add makes it.
+
+    Raises:
+        ContractError: as ``rms_norm_q8``, or where ``x`` is not float32 or ``r`` has another shape.
+    """
+    _check_norm(x, weight, "8-bit RMSNorm")
+    require_cuda("8-bit RMSNorm", x, r=r)
+    if x.dtype != torch.float32:
+        msg = f"x: dtype must be {torch.float32} (the residual stream), got {x.dtype}"
+        raise ContractError(msg)
+    if r.shape != x.shape:
+        msg = f"r: expected shape {tuple(x.shape)}, got {tuple(r.shape)}"
+        raise ContractError(msg)
+    if r.dtype not in SUPPORTED:
+        msg = f"r: dtype must be one of {SUPPORTED}, got {r.dtype}"
+        raise ContractError(msg)
+    return _norm(x, r.contiguous(), weight, floor, eps)
+
+
+def quantize_rows_q8(x: Tensor, *, relu_square: bool = False) -> tuple[Tensor, Tensor]:
+    """``(q [..., W] int8, scale [...] float32)`` of ``x``'s rows, or of ``relu(x)^2`` (formed in float32).
+
+    ``x`` may be a slice of wider rows (contiguous channels); anything else is copied first.
+
+    Raises:
+        ContractError: on a CPU tensor, an unsupported dtype or rows without channels.
+    """
+    require_cuda("8-bit rows", x)
+    serving_only("8-bit quantisation", x)
+    if x.dtype not in SUPPORTED:
+        msg = f"x: dtype must be one of {SUPPORTED}, got {x.dtype}"
+        raise ContractError(msg)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        msg = f"x: expected rows of at least one channel, got shape {tuple(x.shape)}"
+        raise ContractError(msg)
+    width = x.shape[-1]
+    if not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= width):
+        x = x.contiguous()
+    ldx = x.stride(0) if x.dim() == 2 and x.shape[0] > 1 else width
+    q, scale, pitch = _codes(x)
+    _lib.call(
+        "vb_quantize_rows_q8", x.data_ptr(), ldx, q.data_ptr(), pitch, scale.data_ptr(), x.numel() // width, width,
+        int(relu_square), _lib.DTYPE_CODE[x.dtype], _lib.stream(x.device),
+    )  # fmt: skip
+    return q, scale
+
+
+def _pitched(t: Tensor) -> tuple[Tensor, int]:
+    """``t [rows, K]`` int8 with rows a multiple of 16 bytes apart from a 16-byte boundary, and their
+    pitch: ``t`` itself where it is laid out so (as this module's codes are), else a copy."""
+    k = t.shape[-1]
+    if t.stride(1) == 1 or k == 1:
+        pitch = t.stride(0) if t.shape[0] > 1 else -(-k // 16) * 16
+        if pitch % 16 == 0 and pitch >= k and t.data_ptr() % 16 == 0:
+            return t, pitch
+    pitch = -(-k // 16) * 16
+    copy = torch.zeros(t.shape[0], pitch, dtype=torch.int8, device=t.device)
+    copy[:, :k] = t
+    return copy, pitch
+
+
+def dequantize_rows_q8(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.float32) -> Tensor:
+    """The values ``q * scale`` of 8-bit rows ``[..., W]`` in ``dtype``, rounded once.
+
+    Raises:
+        ContractError: on a CPU tensor, codes that are not int8, scales that are not float32 of the
+            rows' shape or an unsupported ``dtype``.
+    """
+    require_cuda("8-bit rows", q, scale=scale)
+    if q.dtype != torch.int8 or scale.dtype != torch.float32:
+        msg = f"q, scale: dtypes must be {torch.int8} and {torch.float32}, got {q.dtype} and {scale.dtype}"
+        raise ContractError(msg)
+    if q.dim() < 1 or q.shape[:-1] != scale.shape or q.shape[-1] < 1:
+        msg = f"scale: expected one per row of q {tuple(q.shape)}, got shape {tuple(scale.shape)}"
+        raise ContractError(msg)
+    if dtype not in SUPPORTED:
+        msg = f"dtype: must be one of {SUPPORTED}, got {dtype}"
+        raise ContractError(msg)
+    width = q.shape[-1]
+    rows = q.numel() // width
+    flat = q.reshape(rows, width)  # a view of codes as this module lays them out
+    if (width > 1 and flat.stride(1) != 1) or (rows > 1 and flat.stride(0) < width):
+        flat = flat.contiguous()
+    y = torch.empty(q.shape, dtype=dtype, device=q.device)
+    _lib.call(
+        "vb_dequantize_rows_q8", flat.data_ptr(), flat.stride(0) if rows > 1 else width,
+        scale.contiguous().data_ptr(), y.data_ptr(), rows, width, _lib.DTYPE_CODE[dtype], _lib.stream(q.device),
+    )  # fmt: skip
+    return y
+
+
+def linear_q8(xq: Tensor, xs: Tensor, wq: Tensor, ws: Tensor, out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """``y [..., N]``: the quantised linear layer, ``y[m, n] = (sum_k xq[m, k] wq[n, k]) * xs[m] * ws[n]``.
+
+    Args:
+        xq, xs: int8 rows ``[..., K]`` and their float32 scales ``[...]``.
+        wq, ws: int8 weights ``[N, K]`` and their float32 scales ``[N]``.
+        out_dtype: float32, bf16 or f16; the scaled float32 sum is rounded to it once.
+
+    Raises:
+        ContractError: on a shape or dtype mismatch, a CPU tensor or ``K`` above 131056 (where a sum
+            of int8 products may leave int32).
+    """
+    dims: Dims = {}
+    check_shape("wq", wq, ("N", "K"), dims, torch.int8)
+    check_shape("ws", ws, ("N",), dims, torch.float32)
+    if xq.dim() < 1 or xq.dtype != torch.int8 or xq.shape[-1] != dims["K"]:
+        msg = f"xq: expected int8 rows of {dims['K']} channels, got {xq.dtype} {tuple(xq.shape)}"
+        raise ContractError(msg)
+    if xs.shape != xq.shape[:-1] or xs.dtype != torch.float32:
+        msg = f"xs: expected one float32 scale per row of xq {tuple(xq.shape)}, got {xs.dtype} {tuple(xs.shape)}"
+        raise ContractError(msg)
+    if out_dtype not in SUPPORTED:
+        msg = f"out_dtype: must be one of {SUPPORTED}, got {out_dtype}"
+        raise ContractError(msg)
+    require_cuda("int8 product", xq, xs=xs, wq=wq, ws=ws)
+    n, k = dims["N"], dims["K"]
+    if n < 1 or not 1 <= k <= MAX_K:
+        msg = f"wq: expected at least one row of 1 to {MAX_K} channels, got shape {tuple(wq.shape)}"
+        raise ContractError(msg)
+    flat = xq if xq.dim() == 2 else xq.reshape(-1, k)
+    rows, ldx = _pitched(flat)
+    weights, ldw = _pitched(wq)
+    m = flat.shape[0]
+    y = torch.empty(*xq.shape[:-1], n, dtype=out_dtype, device=xq.device)
+    _lib.call(
+        "vb_linear_q8", rows.data_ptr(), ldx, xs.contiguous().data_ptr(), weights.data_ptr(), ldw,
+        ws.contiguous().data_ptr(), y.data_ptr(), m, n, k, _lib.DTYPE_CODE[out_dtype],
+        _lib.status_word(xq.device).data_ptr(), _lib.stream(xq.device),
+    )  # fmt: skip
+    return y
