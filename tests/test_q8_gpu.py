@@ -185,7 +185,8 @@ def _assert_product(y: torch.Tensor, xq, xs, wq, ws) -> None:
     ("m", "n", "k"),
     [(1, 1, 1), (1, 16, 32), (1, 1544, 512), (2, 8, 16), (7, 130, 48), (16, 128, 128), (17, 129, 144), (33, 300, 272),
      (64, 512, 1536), (64, 1544, 512), (65, 96, 4096), (100, 1000, 1000), (127, 255, 129), (128, 256, 256),
-     (129, 257, 640), (200, 2001, 1040), (300, 64, 64), (257, 513, 8), (512, 512, 2048), (1000, 777, 130)],
+     (129, 257, 640), (200, 2001, 1040), (300, 64, 64), (257, 513, 8), (512, 512, 2048), (1000, 777, 130),
+     (1300, 4100, 1040), (2200, 1290, 520), (700, 4160, 2304)],
 )  # fmt: skip
 def test_the_product(m: int, n: int, k: int, dtype: torch.dtype) -> None:
     xq, xs, wq, ws = _operands(m, n, k, 14)
