@@ -13,7 +13,7 @@ __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.la
 
 template <typename K, typename... P>
 int launch_early(const char* what, K kernel, dim3 grid, int threads, int smem, int cluster, cudaStream_t st, P... args) {
-  if (smem > 48 * 1024)
+  if (smem > 32 * 1024)  // with the kernel's static arrays this may pass the 48 KB a launch has by default
     VB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -28,7 +28,12 @@ int launch_early(const char* what, K kernel, dim3 grid, int threads, int smem, i
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  VB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // reported here, not again by the next launch's check
+    set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
+    return VB_ERR_CUDA;
+  }
   count_launch();
   return VB_OK;
 }
