@@ -420,7 +420,7 @@ VB_API int vb_linear_q8(const int8_t *xq, int64_t ldx, const float *xs, const in
  * [B, HKV, DK] (row strides in elements), pos [B]: the token is written and attends the slots with
  * p - W < pos <= p, itself included, as the ring holds them (scale 1/sqrt(DK), head h reading key
  * head h / (H / HKV)); o [B, H, DK], zero in a row whose position is negative (which writes nothing).
- * `workspace`: vb_q4_attend_workspace bytes; `status` as in vb_linear_q8. */
+ * `workspace`: vb_q4_attend_workspace bytes, 16-byte aligned. */
 VB_API int vb_q4_write(void *k_codes, void *k_params, void *v_codes, void *v_params,
                        int64_t *ring_pos, const void *k, int64_t k_batch, int64_t k_token,
                        const void *v, int64_t v_batch, int64_t v_token, const int64_t *pos, int B,
@@ -434,7 +434,7 @@ VB_API int vb_q4_attend(const void *q, int64_t q_row, const void *k_new, int64_t
                         const void *v_new, int64_t v_row, const int64_t *pos, void *k_codes,
                         void *k_params, void *v_codes, void *v_params, int64_t *ring_pos, void *o,
                         void *workspace, int B, int H, int HKV, int DK, int W, int SLOTS, int dtype,
-                        int *status, void *stream);
+                        void *stream);
 
 #ifdef __cplusplus
 }

@@ -37,6 +37,6 @@ def test_the_4_bit_cache_entry_points_refuse_bad_arguments_without_a_gpu() -> No
     _refused("vb_q4_read", *ring, None, None, None, None, 1, 1, 1, 64, 64, 100, 0, None, match="multiple of 64")
     _refused("vb_q4_read", *ring, None, None, None, None, 1, 1, 1, 64, 64, 64, 9, None, match="dtype code 9")
     attend = [None, 0, None, 0, None, 0, None, *ring, None, None]
-    _refused("vb_q4_attend", *attend, 1, 3, 2, 64, 64, 64, 0, None, None, match="not a multiple of 2 key heads")
-    _refused("vb_q4_attend", *attend, 1, 2, 2, 64, 64, 64, 0, None, None, match="null pointer")
+    _refused("vb_q4_attend", *attend, 1, 3, 2, 64, 64, 64, 0, None, match="not a multiple of 2 key heads")
+    _refused("vb_q4_attend", *attend, 1, 2, 2, 64, 64, 64, 0, None, match="null pointer")
     assert _lib.query("vb_q4_attend_workspace", 1, 8, 2, 64, 4096) >= 16

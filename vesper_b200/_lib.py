@@ -80,7 +80,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vb_q4_write": (_I, [_P] * 6 + [_I64, _I64, _P, _I64, _I64, _P] + [_I] * 7 + [_P]),
     "vb_q4_read": (_I, [_P] * 9 + [_I] * 7 + [_P]),
     "vb_q4_attend_workspace": (_SZ, [_I, _I, _I, _I, _I]),
-    "vb_q4_attend": (_I, [_P, _I64, _P, _I64, _P, _I64] + [_P] * 8 + [_I] * 7 + [_P, _P]),
+    "vb_q4_attend": (_I, [_P, _I64, _P, _I64, _P, _I64] + [_P] * 8 + [_I] * 7 + [_P]),
     "vb_residual_add": (_I, [_P, _P, _P, _P, ctypes.c_longlong, _I, _I, _P]),
     "vb_residual_add_bwd": (_I, [_P, _P, _P, _P, ctypes.c_longlong, _I, _I, _P]),
 }

@@ -5,17 +5,20 @@
 // The bytes of the cache bound it: 0.625 per channel at DK a multiple of 32, which at the memory's rate
 // leaves some three instructions per channel on the ordinary pipes, less than unpacking and one
 // product per head would take. So the codes go to the matrix units as they are. A warp takes tiles of
-// 64 slots (copied by the bulk engine, two tiles in flight per warp) and eight query heads of one key head:
+// 64 slots (copied 16 bytes a lane by cp.async, two tiles in flight per warp) and eight query heads of one key head:
 //   scores  S[slot, head] = sum_g step[slot, g] (sum_{c in g} code q) + lo[slot, g] (sum_{c in g} q):
 //     m16n8k16 in f16, slots as rows. A code in the low four bits of a half is the subnormal code 2^-24, one
 //     in the next four bits 16 code 2^-24, both exact, so a word of eight codes needs one shift and
 //     four ANDs; the queries are scaled per head by a power of two to fit f16 (an f32 query takes two terms) and
 //     divided by 16 where their codes come 16-fold. The group's step and lo are applied to the float32 sums.
-//   output  O[channel, head] = sum_slot (w step) (code - 8) + w (lo + 8 step): m16n8k16 in bf16 (whose range the
-//     products w step need), channels as rows. A code becomes a bf16 number by OR (128 + code) and one subtraction
-//     per pair; centred codes keep the rounding of w step and of the sums in proportion to the values. The weights cross from the scores' layout to the operand's by movmatrix. w step is rounded to
-//     bf16 for bf16 and f16 inputs (2^-9, of both signs) and held in three bf16 terms for float32.
-// Running maximum and sum per warp and head in float32; the warps' parts are joined in shared memory, those of the
+//   output  O[channel, head] = sum_slot (w step) code + w lo: m16n8k16 in f16, channels as rows, the codes again as
+//     they are (those in the upper four bits make their rows of O 16-fold, taken off at the end). The products w step
+//     are rounded to f16 (2^-12 of each, of both signs), whose range they fit because the scores' reference is chosen
+//     with the largest step in view. They cross from the scores' layout to the operand's by movmatrix. For float32
+//     they are held in three bf16 terms and the codes as bf16 code - 8, one OR and one subtraction per pair: sums of
+//     numbers around zero, which the matrix unit's float32 sums keep to 1e-6 of the output.
+// A reference r and the sum of the weights 2^(score - r) per warp and head in float32; r rises only when a weight times
+// the largest step of its tile would pass 2^14, and then to 2^6, so that the sums are seldom rescaled. The warps' parts are joined in shared memory, those of the
 // CTAs that share a long window by a second kernel, in a fixed order. A slot that is not seen has score -inf and its
 // step and lo are read as zeros, whatever it holds.
 #include <cmath>
@@ -28,18 +31,24 @@
 namespace vb {
 namespace {
 
-constexpr int AW = 8;  // warps per CTA
 constexpr int HEADS = 8;  // query heads of one key head per CTA
+
+// resident CTAs: registers for DK above 64 leave room for one
+__host__ __device__ constexpr int ctas_per_sm(int dk) { return dk <= 64 ? 2 : 1; }
 
 template <typename T, int DK>
 struct Q4Attn {
   static constexpr int GS = q4_group(DK), NG = DK / GS;
   static constexpr int CODES = DK / 2, PAR = NG * 4;  // bytes per slot
-  static constexpr int VC = Q4_TILE * CODES, KP = 2 * VC, VP = KP + Q4_TILE * PAR, POS = VP + Q4_TILE * PAR;
-  static constexpr int TILE = POS + Q4_TILE * 8;
-  static constexpr int STAGES = 2;
+  static constexpr int TS = Q4_TILE, MT = TS / 16;     // slots of a warp's tile, and its steps of 16
+  static constexpr int VC = TS * CODES, KP = 2 * VC, VP = KP + TS * PAR, POS = VP + TS * PAR;
+  static constexpr int TILE = POS + TS * 8;
+  static constexpr int AW = 8, STAGES = 2, CTAS = ctas_per_sm(DK);  // warps per CTA, tiles in flight per warp
   static constexpr int SMEM = AW * STAGES * TILE;
-  static constexpr int QT = sizeof(T) == 4 ? 2 : 1, PT = sizeof(T) == 4 ? 3 : 1;  // terms of queries, of weights
+  static constexpr int QT = sizeof(T) == 4 ? 2 : 1;  // f16 terms of a query
+  static constexpr int PT = sizeof(T) == 4 ? 3 : 1;              // terms of a weight's product: one f16, or three bf16
+  // the sum of lo times the queries' sums as one product in bf16: four groups, two terms
+  static constexpr bool LO_MMA = QT == 1 && (NG == 1 || NG == 2 || NG == 4);
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -49,12 +58,31 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ float exp2_approx(float x) {  // within 2^-22; 0 for -inf
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -72,6 +100,13 @@ __device__ __forceinline__ uint32_t centred(uint32_t x) {
   uint32_t y;
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"((x & 0x000f000fu) | 0x43004300u), "r"(0x43084308u));
   return y;
+}
+
+// the larger of two pairs of bf16 numbers, each half for itself; a NaN gives way to a number
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t x, uint32_t y) {
+  uint32_t z;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+  return z;
 }
 
 // BYTES consecutive bytes (aligned to their largest power-of-two divisor, 16 at most) as words
@@ -107,63 +142,199 @@ struct Ring {
   int64_t* pos;
 };
 
-// Partial layout: [(b * units + unit) * splits + z][HEADS][DK + 2], per head the unnormalised output, the base-2
-// running maximum and the sum.
-template <typename T, int DK>
-__global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
-    q4_attn_kernel(const T* __restrict__ q, int64_t q_row, const T* __restrict__ k_new, int64_t k_row,
-                   const T* __restrict__ v_new, int64_t v_row, const int64_t* __restrict__ pos, Ring ring,
-                   T* __restrict__ o, float* __restrict__ part, int H, int HKV, int head_tiles, int W, int SLOTS,
-                   float scale_log2, int* status) {
-  using C = Q4Attn<T, DK>;
-  constexpr int GS = C::GS, NG = C::NG, QT = C::QT, PT = C::PT, TILES = DK / 16, KSTEPS = GS / 16;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[AW][C::STAGES];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int z = blockIdx.x, splits = gridDim.x, unit = blockIdx.y, kh = unit / head_tiles, ht = unit - kh * head_tiles;
-  const int64_t b = blockIdx.z;
-  const int G = H / HKV, h0 = kh * G + ht * HEADS, heads = min(HEADS, G - ht * HEADS);
-  uint8_t* mine = smem + warp * C::STAGES * C::TILE;
-  if (lane == 0) {
-    for (int i = 0; i < C::STAGES; ++i) mbar_init(&full[warp][i], 1);
-    mbar_fence_init();
+// tiles of a row that can be seen from position p
+template <int TS>
+__device__ __forceinline__ int tiles_of(int64_t p, int W) {
+  return p < 0 ? 0 : (int)((min(p + 1, (int64_t)W) + TS - 1) / TS);
+}
+
+// Where tile `at` of all rows' and units' tiles lies, in that order: its row, the row's first tile and number of
+// tiles (per unit). Called by whole warps.
+template <int TS>
+__device__ __forceinline__ void find_row(const int64_t* pos, int B, int units, int W, int64_t at, int64_t& row,
+                                         int64_t& first, int& n) {
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  for (int r0 = 0; r0 < B; r0 += 32) {
+    const int mine = r0 + lane < B ? tiles_of<TS>(pos[r0 + lane], W) : 0;
+    int upto = mine;  // 32 rows of at most 2^25 tiles
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, x);
+      if (lane >= x) upto += y;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * units > at);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      row = r0 + l;
+      n = __shfl_sync(0xffffffffu, mine, l);
+      first = (before + __shfl_sync(0xffffffffu, upto, l) - n) * units;
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  __syncwarp();
+  row = B;
+  first = before * units;
+  n = 0;
+}
+
+// All rows' and units' tiles, and how many of a launch's CTAs share them: as many as have a tile for each of their warps,
+// but one for each unit that sees something if that is more.
+template <int TS, int AW>
+__device__ __forceinline__ int64_t all_tiles(const int64_t* pos, int B, int units, int W, int& ctas) {
+  int64_t sum = 0;
+  int live = 0;
+  for (int r = threadIdx.x & 31; r < B; r += 32) {
+    const int n = tiles_of<TS>(pos[r], W);
+    sum += n;
+    live += n > 0;
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+  live = __reduce_add_sync(0xffffffffu, live);
+  sum *= units;
+  ctas = (int)min((int64_t)ctas, max((sum + AW - 1) / AW, (int64_t)live * units));
+  return sum;
+}
+
+// `total` tiles in even parts: part i begins at floor(i total / parts)
+struct Share {
+  int64_t each;
+  uint32_t rest, parts;
+  __device__ __forceinline__ Share(int64_t total, int n) : parts((uint32_t)n) {
+    if (total < ((int64_t)1 << 32)) {
+      each = (uint32_t)total / parts;
+      rest = (uint32_t)total % parts;
+    } else {
+      each = total / n;
+      rest = (uint32_t)(total % n);
+    }
+  }
+  __device__ __forceinline__ int64_t start(uint32_t i) const { return each * i + rest * i / parts; }
+};
+
+// A unit is eight query heads of one key head. With `shared` the CTAs divide all rows' and units' tiles evenly between
+// them, whatever the rows' lengths: CTA i takes tiles [i T / n, (i + 1) T / n) and writes what it has of a unit it does
+// not hold whole to its partials, [2 i] of the unit it starts within and [2 i + 1] of the one it ends within, each
+// [HEADS][DK + 2]: per head the unnormalised output, the reference and the sum; span[row][unit] gets the first and
+// the last CTA of a unit. Else a CTA per unit and row.
+template <typename T, int DK>
+__global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
+    q4_attn_kernel(const T* __restrict__ q, int64_t q_row, int q_vec, const T* __restrict__ k_new, int64_t k_row,
+                   const T* __restrict__ v_new, int64_t v_row, const int64_t* __restrict__ pos, Ring ring,
+                   T* __restrict__ o, float* __restrict__ part, int2* __restrict__ span, int shared, int B, int H, int HKV, int head_tiles, int W,
+                   int SLOTS, float scale_log2) {
+  using C = Q4Attn<T, DK>;
+  constexpr int GS = C::GS, NG = C::NG, QT = C::QT, PT = C::PT, TILES = DK / 16, KSTEPS = GS / 16, AW = C::AW;
+  constexpr int TS = C::TS, MT = C::MT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int units = HKV * head_tiles, G = H / HKV;
+  uint8_t* mine = smem + warp * C::STAGES * C::TILE;
   grid_wait();
   grid_release();
-  const int64_t p = pos[b];
-  const int nt = p < 0 ? 0 : (int)((min(p + 1, (int64_t)W) + Q4_TILE - 1) / Q4_TILE);  // tiles that can be seen
-  const int lo_t = (int)((int64_t)nt * z / splits), hi_t = (int)((int64_t)nt * (z + 1) / splits);
+  int64_t b = blockIdx.y, from = 0, until = 1, row_first = 0;  // tiles [from, until) of all, the row's first
+  int n = 0, unit = blockIdx.x, lo_t = 0, hi_t = 0;  // tiles of a unit of row b, and those of them this CTA has
+  if (shared) {
+    int ctas = gridDim.x;
+    const int64_t total = all_tiles<TS, AW>(pos, B, units, W, ctas);
+    if (blockIdx.x >= ctas) return;
+    const Share share(total, ctas);
+    from = share.start(blockIdx.x);
+    until = share.start(blockIdx.x + 1);
+    find_row<TS>(pos, B, units, W, from, b, row_first, n);
+  }
+  while (from < until) {
+  int64_t p = 0;
+  if (shared) {
+    p = pos[b];
+    unit = from - row_first < ((int64_t)1 << 32) ? (int)((uint32_t)(from - row_first) / (uint32_t)n)
+                                                 : (int)((from - row_first) / n);
+    lo_t = (int)(from - row_first - (int64_t)unit * n);
+    hi_t = (int)min((int64_t)n, lo_t + (until - from));
+    from += hi_t - lo_t;
+  } else {
+    hi_t = SLOTS / TS;  // until the position has come: the first copies do not wait for it
+    from = until;
+  }
+  const int kh = unit / head_tiles, ht = unit - kh * head_tiles, h0 = kh * G + ht * HEADS, heads = min(HEADS, G - ht * HEADS);
   const int64_t base = (b * HKV + kh) * SLOTS;
-  const int own = p < 0 ? -1 : (int)(p % W);
-  auto copy = [&](int i) {  // tile lo_t + warp + 8 i into its stage
+  // queries: thread (g, t) holds head g's channels of every group that the key codes of lane part t belong to. They and
+  // the token are loaded before the cache's tiles, behind which they would wait
+  __align__(16) T xraw[NG * (GS / 4)], tokraw[8];  // as they come: nothing waits for them before the copies are issued
+  {
+    const T* src = q + b * q_row + (int64_t)(h0 + min(g, heads - 1)) * DK + t * (GS / 4);
+    constexpr int BYTES = GS / 4 * (int)sizeof(T);
+    if (q_vec) {  // rows on 16-byte boundaries
+#pragma unroll
+      for (int a = 0; a < NG; ++a) {
+        if constexpr (BYTES == 8) reinterpret_cast<uint2*>(xraw)[a] = __ldg(reinterpret_cast<const uint2*>(src + a * GS));
+        else
+#pragma unroll
+          for (int i = 0; i < BYTES / 16; ++i)
+            reinterpret_cast<uint4*>(xraw)[a * (BYTES / 16) + i] = __ldg(reinterpret_cast<const uint4*>(src + a * GS) + i);
+      }
+    } else {
+#pragma unroll
+      for (int a = 0; a < NG; ++a)
+#pragma unroll
+        for (int i = 0; i < GS / 4; ++i) xraw[a * (GS / 4) + i] = src[a * GS + i];
+    }
+  }
+  // the token: lane c < 16 holds eight channels of the key, 16 + c of the value
+  const bool tok_value = lane >= 16;
+  const int tok_c = (lane & 15) * 8;
+  if (tok_c < DK) {
+    const T* src = tok_value ? v_new + b * v_row + (int64_t)kh * DK + tok_c : k_new + b * k_row + (int64_t)kh * DK + tok_c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) tokraw[i] = src[i];
+  }
+  auto copy = [&](int i) {  // tile lo_t + warp + 8 i into stage i mod 2; the group is committed even if it is empty
     const int tile = lo_t + warp + AW * i;
-    if (tile >= hi_t) return;
-    uint8_t* to = mine + (i % C::STAGES) * C::TILE;
-    uint64_t* bar = &full[warp][i % C::STAGES];
-    const int64_t s = base + (int64_t)tile * Q4_TILE;
-    mbar_arrive_expect_tx(bar, C::TILE);
-    bulk_load(to, ring.k_codes + s * C::CODES, C::VC, bar);
-    bulk_load(to + C::KP, ring.k_params + s * NG, Q4_TILE * C::PAR, bar);
-    bulk_load(to + C::POS, ring.pos + b * SLOTS + (int64_t)tile * Q4_TILE, Q4_TILE * 8, bar);
-    bulk_load(to + C::VC, ring.v_codes + s * C::CODES, C::VC, bar);
-    bulk_load(to + C::VP, ring.v_params + s * NG, Q4_TILE * C::PAR, bar);
+    if (tile < hi_t) {
+      const uint32_t to = smem_u32(mine + (i % C::STAGES) * C::TILE) + 16 * lane;
+      const int64_t s0 = base + (int64_t)tile * TS;
+      const uint8_t* kc = ring.k_codes + s0 * C::CODES + 16 * lane;
+      const uint8_t* vc = ring.v_codes + s0 * C::CODES + 16 * lane;
+      const uint8_t* kp = reinterpret_cast<const uint8_t*>(ring.k_params + s0 * NG) + 16 * lane;
+      const uint8_t* vp = reinterpret_cast<const uint8_t*>(ring.v_params + s0 * NG) + 16 * lane;
+#pragma unroll
+      for (int x = 0; x < C::VC; x += 512) cp_async16(to + x, kc + x, 16);
+#pragma unroll
+      for (int x = 0; x < TS * C::PAR; x += 512)
+        if (x + 512 <= TS * C::PAR || x + 16 * lane < TS * C::PAR) {
+          cp_async16(to + C::KP + x, kp + x, 16);
+          cp_async16(to + C::VP + x, vp + x, 16);
+        }
+      cp_async16(to + C::POS, reinterpret_cast<const uint8_t*>(ring.pos + b * SLOTS + (int64_t)tile * TS) + 16 * lane, 16);
+#pragma unroll
+      for (int x = 0; x < C::VC; x += 512) cp_async16(to + C::VC + x, vc + x, 16);
+    }
+    cp_async_commit();
   };
-  if (lane == 0)
-    for (int i = 0; i < C::STAGES; ++i) copy(i);
+#pragma unroll
+  for (int i = 0; i < C::STAGES; ++i) copy(i);
 
-  // queries: thread (g, t) holds head g's channels of every group that the key codes of lane part t belong to
-  uint32_t qb[NG][KSTEPS][QT][2];
+  if (!shared) {
+    p = pos[b];
+    n = hi_t = tiles_of<TS>(p, W);
+  }
+  const int own = p < 0 ? -1 : p < ((int64_t)1 << 31) ? (int)((uint32_t)p % (uint32_t)W) : (int)(p % W);
+  const int own_at = own >= 0 ? own / TS - lo_t : -1;  // the warp whose tile holds the token's slot has it
+  const bool has_own = own_at >= 0 && own / TS < hi_t && own_at % AW == warp;
+
+  uint32_t qb[NG][KSTEPS][QT][2], qlo[2] = {0u, 0u};
   float qs[NG][2], f[2];
   {
     float x[NG][GS / 4], top = 0.f, sum[NG];
 #pragma unroll
     for (int a = 0; a < NG; ++a)
 #pragma unroll
-      for (int i = 0; i < GS / 4; ++i) {
-        x[a][i] = g < heads ? to_f32<T>(q[b * q_row + (int64_t)(h0 + g) * DK + a * GS + t * (GS / 4) + i]) : 0.f;
-        top = fmaxf(top, fabsf(x[a][i]));
-      }
+      for (int i = 0; i < GS / 4; ++i) x[a][i] = g < heads ? to_f32<T>(xraw[a * (GS / 4) + i]) : 0.f;
+#pragma unroll
+    for (int a = 0; a < NG; ++a)
+#pragma unroll
+      for (int i = 0; i < GS / 4; ++i) top = fmaxf(top, fabsf(x[a][i]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // the power of two that brings the largest magnitude to [2^14, 2^15), and its inverse times 2^24
@@ -194,6 +365,15 @@ __global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
         }
       }
     }
+    if constexpr (C::LO_MMA) {
+      // k = 2 t holds a step (times zero), k = 2 t + 1 the lo of group t, times the group's query sum in two terms
+      float mine_sum = 0.f;
+#pragma unroll
+      for (int a = 0; a < NG; ++a) mine_sum = t == a ? sum[a] * 5.9604644775390625e-8f : mine_sum;  // 2^-24
+      const float hi = __bfloat162float(__float2bfloat16_rn(mine_sum));
+      qlo[0] = pack_bf16(0.f, hi);
+      qlo[1] = pack_bf16(0.f, mine_sum - hi);
+    }
     // what the sums' layout needs: heads 2 t and 2 t + 1
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -204,19 +384,44 @@ __global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
     }
   }
 
-  // the new token, in the warp whose tile holds its slot: lane c < 16 holds eight channels of the key, 16 + c of
-  // the value
-  const int own_at = own >= 0 ? own / Q4_TILE - lo_t : -1;
-  const bool has_own = own_at >= 0 && own / Q4_TILE < hi_t && own_at % AW == warp;
-  float tok[8];
-  if (has_own) {
-    const int c = (lane & 15) * 8;
-    const T* src = lane < 16 ? k_new + b * k_row + (int64_t)kh * DK + c : v_new + b * v_row + (int64_t)kh * DK + c;
+  uint32_t tok_codes = 0, tok_params = 0;
+  if (has_own) {  // quantised, and written to the ring once per key head
+    float tok[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) tok[i] = c < DK ? to_f32<T>(src[i]) : 0.f;
+    for (int j = 0; j < 8; ++j) tok[j] = tok_c < DK ? to_f32<T>(tokraw[j]) : 0.f;
+    float lowest = tok[0], highest = tok[0];
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lowest = fminf(lowest, tok[j]);
+      highest = fmaxf(highest, tok[j]);
+      nan |= tok[j] != tok[j];
+    }
+    if (nan) lowest = highest = __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int s = 1; s < GS / 8; s <<= 1) {
+      const float l2 = __shfl_xor_sync(0xffffffffu, lowest, s), h2 = __shfl_xor_sync(0xffffffffu, highest, s);
+      const bool bad = lowest != lowest || l2 != l2;
+      lowest = bad ? __uint_as_float(0x7fc00000u) : fminf(lowest, l2);
+      highest = bad ? lowest : fmaxf(highest, h2);
+    }
+    float step, lo;
+    q4_params(lowest, highest, step, lo);
+    const float inverse = step > 0.f ? 1.0f / step : 0.f;
+    tok_params = q4_pack_params(step, lo);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) tok_codes |= q4_code(tok[j], step, lo, inverse) << (4 * j);
+    if (tok_c < DK && ht == 0) {
+      uint8_t* out = (tok_value ? ring.v_codes : ring.k_codes) + (base + own) * C::CODES;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        out[(tok_value ? q4_value_place(DK, tok_c + 2 * j) : q4_key_place(DK, tok_c + 2 * j)) / 2] = (uint8_t)(tok_codes >> (8 * j));
+      if (tok_c % GS == 0) (tok_value ? ring.v_params : ring.k_params)[(base + own) * NG + tok_c / GS] = tok_params;
+    }
+    if (unit == 0 && lane == 0) ring.pos[b * SLOTS + own] = p;
   }
 
-  float acc[TILES][4], low[NG][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float acc[TILES][4], low[NG][2], ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < TILES; ++i)
 #pragma unroll
@@ -228,70 +433,49 @@ __global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
   const int krow = g ^ ((g >> 2) & 1), vrow0 = (2 * t) ^ (t >> 1), vrow1 = (2 * t + 1) ^ (t >> 1);
 
   for (int i = 0; lo_t + warp + AW * i < hi_t; ++i) {
-    const int st = i % C::STAGES, tile = lo_t + warp + AW * i;
-    uint8_t* at = mine + st * C::TILE;
-    const bool landed = mbar_wait(&full[warp][st], (i / C::STAGES) & 1);
-    if (!__all_sync(0xffffffffu, landed)) {
-      if (lane == 0) atomicOr(status, 1);
-      for (int j = i; j < i + C::STAGES && lo_t + warp + AW * j < hi_t; ++j)  // the copies that may still be in flight
-        mbar_wait(&full[warp][j % C::STAGES], (j / C::STAGES) & 1, 200000000ull);
-      break;
-    }
-    if (has_own && own_at == warp + AW * i) {
-      // quantise the token and put it into its slot, here and (once per key head) in the ring
-      const bool value = lane >= 16;
-      const int c = (lane & 15) * 8, slot = own % Q4_TILE;
-      float lowest = tok[0], highest = tok[0];
-      bool nan = false;
+    const int tile = lo_t + warp + AW * i;
+    uint8_t* at = mine + (i % C::STAGES) * C::TILE;
+    cp_async_wait<C::STAGES - 1>();
+    __syncwarp();
+    if (has_own && own_at == warp + AW * i) {  // the token takes its slot here too
+      if (tok_c < DK) {
+        const int slot = own % TS;
+        uint8_t* codes = at + (tok_value ? C::VC : 0) + slot * C::CODES;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        lowest = fminf(lowest, tok[j]);
-        highest = fmaxf(highest, tok[j]);
-        nan |= tok[j] != tok[j];
+        for (int j = 0; j < 4; ++j)
+          codes[(tok_value ? q4_value_place(DK, tok_c + 2 * j) : q4_key_place(DK, tok_c + 2 * j)) / 2] =
+              (uint8_t)(tok_codes >> (8 * j));
+        if (tok_c % GS == 0)
+          reinterpret_cast<uint32_t*>(at + (tok_value ? C::VP : C::KP))[slot * NG + tok_c / GS] = tok_params;
       }
-      if (nan) lowest = highest = __uint_as_float(0x7fc00000u);
-#pragma unroll
-      for (int s = 1; s < GS / 8; s <<= 1) {
-        const float l2 = __shfl_xor_sync(0xffffffffu, lowest, s), h2 = __shfl_xor_sync(0xffffffffu, highest, s);
-        const bool bad = lowest != lowest || l2 != l2;
-        lowest = bad ? __uint_as_float(0x7fc00000u) : fminf(lowest, l2);
-        highest = bad ? lowest : fmaxf(highest, h2);
-      }
-      float step, lo;
-      q4_params(lowest, highest, step, lo);
-      const float inverse = step > 0.f ? 1.0f / step : 0.f;
-      if (c < DK) {
-        uint8_t* codes = at + (value ? C::VC : 0) + slot * C::CODES;
-        uint8_t* out = (value ? ring.v_codes : ring.k_codes) + (base + own) * C::CODES;
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          const uint8_t byte = (uint8_t)(q4_code(tok[j], step, lo, inverse) | q4_code(tok[j + 1], step, lo, inverse) << 4);
-          const int place = (value ? q4_value_place(DK, c + j) : q4_key_place(DK, c + j)) / 2;
-          codes[place] = byte;
-          if (ht == 0) out[place] = byte;
-        }
-        if (c % GS == 0) {
-          const uint32_t word = q4_pack_params(step, lo);
-          reinterpret_cast<uint32_t*>(at + (value ? C::VP : C::KP))[slot * NG + c / GS] = word;
-          if (ht == 0) (value ? ring.v_params : ring.k_params)[(base + own) * NG + c / GS] = word;
-        }
-      }
-      if (unit == 0 && lane == 0) ring.pos[b * SLOTS + own] = p;
-      fence_async_smem();  // before the stage is copied into again
       __syncwarp();
     }
-    // which of the 64 slots are seen
-    uint32_t seen[2];
+    // which of the slots are seen
+    uint32_t seen[TS / 32];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int slot = tile * Q4_TILE + 32 * j + lane;
+    for (int j = 0; j < TS / 32; ++j) {
+      const int slot = tile * TS + 32 * j + lane;
       const int64_t kp = reinterpret_cast<const int64_t*>(at + C::POS)[32 * j + lane];
-      seen[j] = __ballot_sync(0xffffffffu, slot == own || (slot < W && kp >= 0 && kp <= p && kp > p - W));
+      seen[j] = __ballot_sync(0xffffffffu, slot == own || (slot < W && kp >= 0 && (uint64_t)(p - kp) < (uint64_t)W));
     }
-    // scores of slots (rows) by heads (columns), in base 2
-    float s[4][4];
+    bool every = true;
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
+    for (int j = 0; j < TS / 32; ++j) every &= seen[j] == 0xffffffffu;
+    if (!every) {  // a slot that is not seen has step and lo 0, whatever it holds
+#pragma unroll
+      for (int x = 0; x < TS * NG / 32; ++x) {
+        const int slot = (32 * x + lane) / NG;
+        if (!((seen[slot >> 5] >> (slot & 31)) & 1u)) {
+          reinterpret_cast<uint32_t*>(at + C::KP)[32 * x + lane] = 0;
+          reinterpret_cast<uint32_t*>(at + C::VP)[32 * x + lane] = 0;
+        }
+      }
+      __syncwarp();
+    }
+    // scores of slots (rows) by heads (columns), to be multiplied by f
+    float s[MT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
       const int r0 = 16 * mt + krow;
       uint32_t c0[(DK / 8 + 3) / 4], c1[(DK / 8 + 3) / 4], p0[NG], p1[NG];
       load_bytes<DK / 8>(at + r0 * C::CODES + t * (DK / 8), c0);
@@ -299,9 +483,22 @@ __global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
       load_bytes<4 * NG>(at + C::KP + r0 * C::PAR, p0);
       load_bytes<4 * NG>(at + C::KP + (r0 + 8) * C::PAR, p1);
       float tot[4] = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (C::LO_MMA) {
+        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at + C::KP + r0 * C::PAR + 4 * (t % NG));
+        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + C::KP + (r0 + 8) * C::PAR + 4 * (t % NG));
+        mma_bf16_first(tot, w0, w1, w0, w1, qlo[0], qlo[1]);
+      } else {
+#pragma unroll
+        for (int a = 0; a < NG; ++a) {
+          tot[0] = fmaf(q4_lo(p0[a]), qs[a][0], tot[0]);
+          tot[1] = fmaf(q4_lo(p0[a]), qs[a][1], tot[1]);
+          tot[2] = fmaf(q4_lo(p1[a]), qs[a][0], tot[2]);
+          tot[3] = fmaf(q4_lo(p1[a]), qs[a][1], tot[3]);
+        }
+      }
 #pragma unroll
       for (int a = 0; a < NG; ++a) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        float d[4];
         uint32_t w0, w1;
         if constexpr (GS == 32) {
           w0 = c0[a]; w1 = c1[a];
@@ -314,51 +511,79 @@ __global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
 #pragma unroll
         for (int k = 0; k < KSTEPS; ++k) {
           const uint32_t x0 = w0 >> (8 * k), x1 = w1 >> (8 * k);
+          const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
 #pragma unroll
-          for (int r = 0; r < QT; ++r)
-            mma_f16(d, x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, qb[a][k][r][0],
-                    qb[a][k][r][1]);
+          for (int r = 0; r < QT; ++r) {
+            if (k == 0 && r == 0) mma_f16_first(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+            else mma_f16(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+          }
         }
-        tot[0] = fmaf(q4_step(p0[a]), d[0], fmaf(q4_lo(p0[a]), qs[a][0], tot[0]));
-        tot[1] = fmaf(q4_step(p0[a]), d[1], fmaf(q4_lo(p0[a]), qs[a][1], tot[1]));
-        tot[2] = fmaf(q4_step(p1[a]), d[2], fmaf(q4_lo(p1[a]), qs[a][0], tot[2]));
-        tot[3] = fmaf(q4_step(p1[a]), d[3], fmaf(q4_lo(p1[a]), qs[a][1], tot[3]));
+        const float s0 = q4_step(p0[a]), s1 = q4_step(p1[a]);
+        tot[0] = fmaf(s0, d[0], tot[0]);
+        tot[1] = fmaf(s0, d[1], tot[1]);
+        tot[2] = fmaf(s1, d[2], tot[2]);
+        tot[3] = fmaf(s1, d[3], tot[3]);
       }
-      const uint32_t bits = seen[mt >> 1] >> (16 * (mt & 1) + krow);
-      s[mt][0] = bits & 1u ? tot[0] * f[0] : -INFINITY;
-      s[mt][1] = bits & 1u ? tot[1] * f[1] : -INFINITY;
-      s[mt][2] = bits & 256u ? tot[2] * f[0] : -INFINITY;
-      s[mt][3] = bits & 256u ? tot[3] * f[1] : -INFINITY;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[mt][x] = tot[x];
     }
-    // the running maximum and sum, and the weights
+    if (!every) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float top = -INFINITY;
+      for (int mt = 0; mt < MT; ++mt) {
+        const uint32_t bits = seen[mt >> 1] >> (16 * (mt & 1) + krow);
+        if (!(bits & 1u)) s[mt][0] = s[mt][1] = -INFINITY;
+        if (!(bits & 256u)) s[mt][2] = s[mt][3] = -INFINITY;
+      }
+    }
+    // the references, the weights and their sum
+    {
+      uint32_t big = 0;
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) top = fmaxf(top, fmaxf(s[mt][c], s[mt][2 + c]));
+      for (int x = 0; x < TS * NG / 32; ++x) big = max_bf16x2(big, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane]);
+      big = __reduce_max_sync(0xffffffffu, big << 16);  // the largest step, below 2^size
+      const float size = (float)max((int)(big >> 23) - 126, -104);
+      float top[2];
+      bool rise = false;
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      top = fmaxf(top, m[c]);
-      const float from = top == -INFINITY ? 0.f : top, fade = exp2f(m[c] - from);
-      m[c] = top;
-      l[c] *= fade;
+      for (int c = 0; c < 2; ++c) {
+        top[c] = -INFINITY;
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        s[mt][c] = exp2f(s[mt][c] - from);
-        s[mt][2 + c] = exp2f(s[mt][2 + c] - from);
-        l[c] += s[mt][c] + s[mt][2 + c];
+        for (int mt = 0; mt < MT; ++mt) top[c] = fmaxf(top[c], fmaxf(s[mt][c], s[mt][2 + c]));
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
+        top[c] = fmaf(top[c], f[c], size);
+        rise |= top[c] > ref[c] + 14.f;
+      }
+      if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float next = fmaxf(ref[c], top[c] - 6.f);
+          const float fade = next == -INFINITY ? 1.f : exp2_approx(ref[c] - next);
+          ref[c] = next;
+          l[c] *= fade;
+#pragma unroll
+          for (int j = 0; j < TILES; ++j) {
+            acc[j][c] *= fade;
+            acc[j][2 + c] *= fade;
+          }
+#pragma unroll
+          for (int a = 0; a < NG; ++a) low[a][c] *= fade;
+        }
       }
 #pragma unroll
-      for (int j = 0; j < TILES; ++j) {
-        acc[j][c] *= fade;
-        acc[j][2 + c] *= fade;
-      }
+      for (int c = 0; c < 2; ++c) {
+        const float r = ref[c] == -INFINITY ? 0.f : ref[c];
 #pragma unroll
-      for (int a = 0; a < NG; ++a) low[a][c] *= fade;
+        for (int mt = 0; mt < MT; ++mt) {
+          s[mt][c] = exp2_approx(fmaf(s[mt][c], f[c], -r));
+          s[mt][2 + c] = exp2_approx(fmaf(s[mt][2 + c], f[c], -r));
+          l[c] += s[mt][c] + s[mt][2 + c];
+        }
+      }
     }
     // weights x values
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
+    for (int mt = 0; mt < MT; ++mt) {
       constexpr int VB = DK / 16, VW = (VB + 3) / 4;
       const int r0 = 16 * mt + krow;
       uint32_t p0[NG], p1[NG], w[4][VW];
@@ -369,41 +594,51 @@ __global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
       load_bytes<VB>(vc + vrow1 * C::CODES, w[1]);
       load_bytes<VB>(vc + (vrow0 + 8) * C::CODES, w[2]);
       load_bytes<VB>(vc + (vrow1 + 8) * C::CODES, w[3]);
-      const uint32_t bits = seen[mt >> 1] >> (16 * (mt & 1) + krow);
-      const uint32_t on0 = 0u - (bits & 1u), on1 = 0u - ((bits >> 8) & 1u);
 #pragma unroll
       for (int a = 0; a < NG; ++a) {
-        const uint32_t q0 = p0[a] & on0, q1 = p1[a] & on1;  // zeros where the slot is not seen
-        const float mid0 = fmaf(8.f, q4_step(q0), q4_lo(q0)), mid1 = fmaf(8.f, q4_step(q1), q4_lo(q1));
-        low[a][0] = fmaf(s[mt][0], mid0, fmaf(s[mt][2], mid1, low[a][0]));
-        low[a][1] = fmaf(s[mt][1], mid0, fmaf(s[mt][3], mid1, low[a][1]));
-        float e[4] = {s[mt][0] * q4_step(q0), s[mt][1] * q4_step(q0), s[mt][2] * q4_step(q1), s[mt][3] * q4_step(q1)};
+        const float st0 = q4_step(p0[a]), st1 = q4_step(p1[a]);
+        // with codes as code - 8, lo + 8 step takes the place of lo
+        const float lo0 = PT > 1 ? fmaf(8.f, st0, q4_lo(p0[a])) : q4_lo(p0[a]);
+        const float lo1 = PT > 1 ? fmaf(8.f, st1, q4_lo(p1[a])) : q4_lo(p1[a]);
+        low[a][0] = fmaf(s[mt][0], lo0, fmaf(s[mt][2], lo1, low[a][0]));
+        low[a][1] = fmaf(s[mt][1], lo0, fmaf(s[mt][3], lo1, low[a][1]));
+        float e[4] = {s[mt][0] * st0, s[mt][1] * st0, s[mt][2] * st1, s[mt][3] * st1};
+        uint32_t b0[PT], b1[PT];
 #pragma unroll
         for (int r = 0; r < PT; ++r) {
-          const uint32_t e0 = pack_bf16(e[0], e[1]), e1 = pack_bf16(e[2], e[3]);
+          const uint32_t e0 = PT > 1 ? pack_bf16(e[0], e[1]) : pack_f16(e[0], e[1]);
+          const uint32_t e1 = PT > 1 ? pack_bf16(e[2], e[3]) : pack_f16(e[2], e[3]);
+          b0[r] = transpose8(e0);
+          b1[r] = transpose8(e1);
           if constexpr (PT > 1) {
             e[0] -= __uint_as_float(e0 << 16); e[1] -= __uint_as_float(e0 & 0xffff0000u);
             e[2] -= __uint_as_float(e1 << 16); e[3] -= __uint_as_float(e1 & 0xffff0000u);
           }
-          const uint32_t b0 = transpose8(e0), b1 = transpose8(e1);
+        }
 #pragma unroll
-          for (int j = 0; j < GS / 16; ++j) {
-            const int i16 = a * (GS / 16) + j;  // channels [16 i16, 16 i16 + 16): nibbles 2 i16 and 2 i16 + 1
-            const int sh = 8 * (i16 & 1);
-            const uint32_t sel = i16 & 2 ? 0x7632u : 0x5410u;
-            const uint32_t x = __byte_perm(w[0][i16 / 4], w[1][i16 / 4], sel);
-            const uint32_t y = __byte_perm(w[2][i16 / 4], w[3][i16 / 4], sel);
-            mma_bf16(acc[i16], centred(x >> sh), centred(x >> (sh + 4)), centred(y >> sh), centred(y >> (sh + 4)), b0, b1);
+        for (int j = 0; j < GS / 16; ++j) {
+          const int i16 = a * (GS / 16) + j;  // channels [16 i16, 16 i16 + 16): byte i16 of the lanes' parts
+          const uint32_t sel = 0x4400u + 0x1111u * (i16 % 4);
+          // that byte of two slots in the low bytes of the halves: low four bits for rows g, the others for rows g + 8
+          const uint32_t x = __byte_perm(w[0][i16 / 4], w[1][i16 / 4], sel);
+          const uint32_t y = __byte_perm(w[2][i16 / 4], w[3][i16 / 4], sel);
+          if constexpr (PT > 1) {
+            const uint32_t a0 = centred(x), a1 = centred(x >> 4), a2 = centred(y), a3 = centred(y >> 4);
+#pragma unroll
+            for (int r = 0; r < PT; ++r) mma_bf16(acc[i16], a0, a1, a2, a3, b0[r], b1[r]);
+          } else {
+            mma_f16(acc[i16], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, b0[0], b1[0]);
           }
         }
       }
     }
     __syncwarp();
-    if (lane == 0) copy(i + C::STAGES);
+    copy(i + C::STAGES);
   }
 
   // this warp's part: heads 2 t and 2 t + 1, channels 16 i + 2 g and 16 i + 2 g + 1
-  __syncthreads();  // the stages are free
+  cp_async_wait_all();  // also of copies that the position then made needless
+  __syncthreads();      // the stages are free
   float* parts = reinterpret_cast<float*>(smem);  // [AW][HEADS][DK + 2]
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -417,14 +652,21 @@ __global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int a = i / (GS / 16);
-      *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(acc[i][c] + low[a][c], acc[i][2 + c] + low[a][c]);
+      const float x = PT > 1 ? acc[i][c] : acc[i][c] * 16777216.f;        // f16: the codes' 2^-24
+      const float y = PT > 1 ? acc[i][2 + c] : acc[i][2 + c] * 1048576.f;  // and 2^-20
+      *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(x + low[a][c], y + low[a][c]);
     }
     if (g == 0) {
-      row[DK] = m[c];
+      row[DK] = ref[c];
       row[DK + 1] = l[c];
     }
   }
   __syncthreads();
+  const bool whole = lo_t == 0 && hi_t == n;
+  if (shared && threadIdx.x == 0) {
+    if (lo_t == 0) span[b * units + unit].x = blockIdx.x;
+    if (hi_t == n) span[b * units + unit].y = blockIdx.x;
+  }
   for (int e = threadIdx.x; e < heads * DK; e += AW * 32) {
     const int h = e / DK, c = e - h * DK;
     const float* col = parts + h * (DK + 2);
@@ -438,10 +680,10 @@ __global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
       L = fmaf(x[DK + 1], fade, L);
       out = fmaf(x[c], fade, out);
     }
-    if (splits == 1) {
+    if (whole) {
       o[(b * H + h0 + h) * DK + c] = from_f32<T>(p < 0 ? 0.f : out / L);
     } else {
-      float* to = part + (((b * gridDim.y + unit) * splits + z) * HEADS + h) * (DK + 2);
+      float* to = part + (2 * (int64_t)blockIdx.x + (lo_t == 0)) * HEADS * (DK + 2) + h * (DK + 2);
       to[c] = out;
       if (c == 0) {
         to[DK] = M;
@@ -449,38 +691,90 @@ __global__ void __launch_bounds__(AW * 32, DK <= 64 ? 2 : 1)
       }
     }
   }
+  if (from >= until) break;
+  // the next unit: its copies come into what was just read
+  __syncthreads();
+  if (hi_t == n && unit + 1 == units) {  // the next row that sees something
+    row_first += (int64_t)n * units;
+    do n = tiles_of<TS>(pos[++b], W);
+    while (n == 0);
+  }
+  }
 }
 
-// joins the splits of a (row, unit) in order; a row that saw nothing (a negative position) is zero
+// Joins the partials of each (row, unit) that several CTAs of a shared launch have had, in a fixed order; a row that sees
+// nothing (a negative position) is zero. A CTA per head, row and unit, the partials spread over its threads.
+constexpr int JOIN = 512;
 template <typename T, int DK>
-__global__ void __launch_bounds__(DK) q4_attn_join_kernel(const float* __restrict__ part, T* __restrict__ o, int H, int HKV,
-                                                          int head_tiles, int units, int splits) {
+__global__ void __launch_bounds__(JOIN) q4_attn_join_kernel(const int64_t* __restrict__ pos, const float* __restrict__ part,
+                                                           const int2* __restrict__ span, T* __restrict__ o, int H, int HKV,
+                                                           int head_tiles) {
+  constexpr int LANES = JOIN / DK;  // threads per channel
+  __shared__ float tops[JOIN / 32], sums[LANES][DK + 1];
+  const int units = HKV * head_tiles, G = H / HKV, unit = blockIdx.y, kh = unit / head_tiles, ht = unit - kh * head_tiles;
+  const int h = blockIdx.x, tid = threadIdx.x;
+  const int64_t b = blockIdx.z;
+  if (ht * HEADS + h >= G) return;
+  T* out = o + (b * H + kh * G + ht * HEADS + h) * DK;
   grid_wait();
   grid_release();
-  const int unit = blockIdx.y, kh = unit / head_tiles, ht = unit - kh * head_tiles, h = blockIdx.x, c = threadIdx.x;
-  const int64_t b = blockIdx.z;
-  const int G = H / HKV, head = kh * G + ht * HEADS + h;
-  if (ht * HEADS + h >= G) return;
-  const float* from = part + ((b * units + unit) * splits * HEADS + h) * (DK + 2);
-  constexpr int STEP = HEADS * (DK + 2);
-  float M = -INFINITY, L = 0.f, out = 0.f;
-  for (int z = 0; z < splits; ++z) M = fmaxf(M, from[(int64_t)z * STEP + DK]);
-#pragma unroll 4
-  for (int z = 0; z < splits; ++z) {
-    const float* x = from + (int64_t)z * STEP;
-    const float fade = x[DK] == -INFINITY ? 0.f : exp2f(x[DK] - M);
-    L = fmaf(x[DK + 1], fade, L);
-    out = fmaf(x[c], fade, out);
+  const int2 ends = span[b * units + unit];
+  if (pos[b] < 0) {
+    if (tid < DK) out[tid] = from_f32<T>(0.f);
+    return;
   }
-  o[(b * H + head) * DK + c] = from_f32<T>(L == 0.f ? 0.f : out / L);
+  const int lo = ends.x, hi = ends.y;
+  if (lo == hi) return;  // that CTA wrote the output
+  // the first CTA ends within the unit (or with it), the others start within it
+  auto row = [&](int i) { return part + ((2 * (int64_t)i + (i == lo)) * HEADS + h) * (DK + 2); };
+  float top = -INFINITY;
+  for (int i = lo + tid; i <= hi; i += JOIN) top = fmaxf(top, row(i)[DK]);
+  top = warp_max(top);
+  if ((tid & 31) == 0) tops[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < JOIN / 32; ++i) top = fmaxf(top, tops[i]);
+  const int c = tid % DK, lane = tid / DK;
+  float acc = 0.f, L = 0.f;
+  if (lane < LANES) {
+#pragma unroll 4
+    for (int i = lo + lane; i <= hi; i += LANES) {
+      const float* x = row(i);
+      const float fade = x[DK] == -INFINITY ? 0.f : exp2f(x[DK] - top);
+      L = fmaf(x[DK + 1], fade, L);
+      acc = fmaf(x[c], fade, acc);
+    }
+    sums[lane][c] = acc;
+    if (c == 0) sums[lane][DK] = L;
+  }
+  __syncthreads();
+  if (tid < DK) {
+    acc = L = 0.f;
+#pragma unroll
+    for (int i = 0; i < LANES; ++i) {
+      acc += sums[i][c];
+      L += sums[i][DK];
+    }
+    out[c] = from_f32<T>(acc / L);
+  }
 }
 
-// CTAs per (row, unit): enough to fill the SMs some times over, each with work for all its warps
-int split_count(int B, int units, int W) {
-  const int tiles = (W + Q4_TILE - 1) / Q4_TILE;
-  const int64_t want = (4 * 148 + (int64_t)B * units - 1) / ((int64_t)B * units);
-  const int most = (tiles + 2 * AW - 1) / (2 * AW);
-  return (int)(want < most ? want : most);
+int sm_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      v = 148;
+    return v > 0 ? v : 148;
+  }();
+  return n;
+}
+
+// CTAs of a shared launch, 0 for a CTA per row and unit: a window of few tiles is one CTA's work, and many units
+// fill the SMs by themselves
+int shared_ctas(int B, int units, int DK, int W) {
+  const int tiles = (W + Q4_TILE - 1) / Q4_TILE, slots = sm_count() * ctas_per_sm(DK);
+  if (tiles <= 16 || (int64_t)B * units >= 8 * slots) return 0;
+  return slots;
 }
 
 int head_tiles_of(int H, int HKV) { return (H / HKV + HEADS - 1) / HEADS; }
@@ -492,14 +786,15 @@ using namespace vb;
 
 extern "C" size_t vb_q4_attend_workspace(int B, int H, int HKV, int DK, int W) {
   if (B <= 0 || H <= 0 || HKV <= 0 || H % HKV || DK <= 0 || W <= 0) return 16;
-  const int units = HKV * head_tiles_of(H, HKV), splits = split_count(B, units, W);
-  return splits == 1 ? 16 : sizeof(float) * (size_t)B * units * splits * HEADS * (DK + 2);
+  const int units = HKV * head_tiles_of(H, HKV), ctas = shared_ctas(B, units, DK, W);
+  if (ctas == 0) return 16;
+  return sizeof(int2) * (size_t)B * units + sizeof(float) * 2 * (size_t)ctas * HEADS * (DK + 2);
 }
 
 extern "C" int vb_q4_attend(const void* q, int64_t q_row, const void* k_new, int64_t k_row, const void* v_new,
                             int64_t v_row, const int64_t* pos, void* k_codes, void* k_params, void* v_codes,
                             void* v_params, int64_t* ring_pos, void* o, void* workspace, int B, int H, int HKV, int DK,
-                            int W, int SLOTS, int dtype, int* status, void* stream) {
+                            int W, int SLOTS, int dtype, void* stream) {
   VB_REQUIRE(B >= 0 && H >= 1 && HKV >= 1 && W >= 1, "q4_attend: bad shape B=%d H=%d HKV=%d W=%d", B, H, HKV, W);
   VB_REQUIRE(H % HKV == 0, "q4_attend: %d query heads are not a multiple of %d key heads", H, HKV);
   VB_REQUIRE(DK >= 16 && DK <= 128 && DK % 16 == 0, "q4_attend: head dimension %d must be a multiple of 16 up to 128", DK);
@@ -507,25 +802,28 @@ extern "C" int vb_q4_attend(const void* q, int64_t q_row, const void* k_new, int
              SLOTS, Q4_TILE, W);
   VB_REQUIRE(dtype_size(dtype) > 0, "q4_attend: unsupported dtype code %d", dtype);
   if (B == 0) return VB_OK;
-  VB_REQUIRE(q && k_new && v_new && pos && k_codes && k_params && v_codes && v_params && ring_pos && o && workspace && status,
+  VB_REQUIRE(q && k_new && v_new && pos && k_codes && k_params && v_codes && v_params && ring_pos && o && workspace,
              "q4_attend: null pointer");
   VB_REQUIRE(aligned16(k_codes) && aligned16(k_params) && aligned16(v_codes) && aligned16(v_params) && aligned16(ring_pos),
              "q4_attend: the ring's buffers must start on 16-byte boundaries");
-  const int head_tiles = head_tiles_of(H, HKV), units = HKV * head_tiles, splits = split_count(B, units, W);
+  VB_REQUIRE(aligned16(workspace), "q4_attend: the workspace must start on a 16-byte boundary");
+  const int head_tiles = head_tiles_of(H, HKV), units = HKV * head_tiles, ctas = shared_ctas(B, units, DK, W);
   VB_REQUIRE(B <= 65535 && units <= 65535, "q4_attend: %d rows of %d head tiles exceed the grid", B, units);
   const Ring ring{(uint8_t*)k_codes, (uint32_t*)k_params, (uint8_t*)v_codes, (uint32_t*)v_params, ring_pos};
   const float scale_log2 = 1.4426950408889634f / sqrtf((float)DK);
+  const int q_vec = aligned16(q) && (q_row * dtype_size(dtype)) % 16 == 0;
   cudaStream_t st = (cudaStream_t)stream;
-  float* part = (float*)workspace;
+  int2* span = (int2*)workspace;  // first, then the partials
+  float* part = (float*)(span + (ctas ? (size_t)B * units : 0));
   return VB_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     auto run = [&](auto dk) -> int {
       constexpr int D = decltype(dk)::value;
-      int rc = launch_early("q4_attend", q4_attn_kernel<T, D>, dim3(splits, units, B), AW * 32, Q4Attn<T, D>::SMEM, 1, st,
-                            (const T*)q, q_row, (const T*)k_new, k_row, (const T*)v_new, v_row, pos, ring, (T*)o, part, H,
-                            HKV, head_tiles, W, SLOTS, scale_log2, status);
-      if (rc || splits == 1) return rc;
-      return launch_early("q4_attend join", q4_attn_join_kernel<T, D>, dim3(HEADS, units, B), D, 0, 1, st,
-                          (const float*)part, (T*)o, H, HKV, head_tiles, units, splits);
+      int rc = launch_early("q4_attend", q4_attn_kernel<T, D>, ctas ? dim3(ctas) : dim3(units, B), Q4Attn<T, D>::AW * 32,
+                            Q4Attn<T, D>::SMEM, 1, st, (const T*)q, q_row, q_vec, (const T*)k_new, k_row, (const T*)v_new,
+                            v_row, pos, ring, (T*)o, part, span, ctas != 0, B, H, HKV, head_tiles, W, SLOTS, scale_log2);
+      if (rc || ctas == 0) return rc;
+      return launch_early("q4_attend join", q4_attn_join_kernel<T, D>, dim3(HEADS, units, B), JOIN, 0, 1, st, pos,
+                          (const float*)part, (const int2*)span, (T*)o, H, HKV, head_tiles);
     };
     switch (DK) {
       case 16: return run(std::integral_constant<int, 16>{});

@@ -215,6 +215,6 @@ def q4_attend_(q: Tensor, k: Tensor, v: Tensor, pos: Tensor, ring: Q4RingKVCache
     _lib.call(
         "vb_q4_attend", q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
         pos.data_ptr(), *_ring_ptrs(ring), o.data_ptr(), ws.data_ptr(), b, heads, hkv, dk, ring.window, slots,
-        _lib.DTYPE_CODE[q.dtype], _lib.status_word(q.device).data_ptr(), _lib.stream(q.device),
+        _lib.DTYPE_CODE[q.dtype], _lib.stream(q.device),
     )  # fmt: skip
     return o
