@@ -38,13 +38,36 @@ __device__ __forceinline__ int q4_value_place(int dk, int c) {
   return ((c & 15) >> 1) * (dk / 8) + 2 * (c >> 4) + (c & 1);
 }
 
-// a group's step and lo (float values of bf16 numbers) from its extremes
-__device__ __forceinline__ void q4_params(float low, float high, float& step, float& lo) {
-  lo = __bfloat162float(__float2bfloat16_rd(low));
+// the smaller and the larger of two numbers, NaN if either is
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float z;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
+
+// A group's step and lo (float values of bf16 numbers) and the correctly rounded reciprocal of step (0 for step 0) from
+// its extremes. Quotients by Markstein's steps (IBM J. Res. Dev. 34, 1990): with r the rounded reciprocal of d, q = n r
+// and one residual step q + (n - q d) r give the rounded n / d; and one step r + (1 - r d) r from an r within a unit in
+// the last place gives the rounded reciprocal, d not having all its bits set. No operand here leaves the
+// range in which the residuals are exact: spans lie between 2^-100 and 2^128.
+__device__ __forceinline__ void q4_params(float low, float high, float& step, float& lo, float& inverse) {
+  // bf16 is float32's upper half: with its lower half added up or cut off, the next number away from or towards zero
+  const uint32_t bits = __float_as_uint(low);
+  lo = __uint_as_float((bits + ((uint32_t)((int32_t)bits >> 31) & 0xffffu)) & 0xffff0000u);
   const float span = high - lo;
-  step = span < Q4_FLAT ? 0.f : __bfloat162float(__float2bfloat16_ru(span / 15.0f));
-  const bool fine = fabsf(lo) <= 3.4e38f && step <= 3.4e38f;  // false for NaN
-  if (!fine) lo = step = __uint_as_float(0x7fc00000u);
+  constexpr float FIFTEENTH = 1.0f / 15.0f;
+  const float q = __fmul_rn(span, FIFTEENTH);
+  const float exact = __fmaf_rn(__fmaf_rn(-q, 15.0f, span), FIFTEENTH, q);
+  step = span < Q4_FLAT ? 0.f : __uint_as_float((__float_as_uint(exact) + 0xffffu) & 0xffff0000u);
+  if (!(fabsf(lo) <= 3.4e38f && span <= 3.4e38f)) lo = step = __uint_as_float(0x7fc00000u);  // also for a NaN
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(step));
+  inverse = step > 0.f ? __fmaf_rn(__fmaf_rn(-step, r, 1.0f), r, r) : 0.f;
 }
 __device__ __forceinline__ uint32_t q4_pack_params(float step, float lo) {
   return (__float_as_uint(step) >> 16) | (__float_as_uint(lo) & 0xffff0000u);
@@ -52,14 +75,58 @@ __device__ __forceinline__ uint32_t q4_pack_params(float step, float lo) {
 __device__ __forceinline__ float q4_step(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float q4_lo(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
-// the code of x: rint of the correctly rounded quotient (x - lo) / step. With r = 1 / step rounded,
-// q = t r and one residual step q + (t - q step) r is the rounded quotient (Markstein, IBM J. Res.
-// Dev. 34, 1990); step 0 or NaN gives code 0
-__device__ __forceinline__ uint32_t q4_code(float x, float step, float lo, float inverse) {
-  const float t = __fsub_rn(x, lo);
-  const float q = __fmul_rn(t, inverse);
-  const float quotient = __fmaf_rn(__fmaf_rn(-q, step, t), inverse, q);
-  return step > 0.f ? (uint32_t)min(__float2int_rn(quotient), 15) : 0u;
+// two floats side by side: Blackwell's packed float32 arithmetic, each half rounded for itself
+__device__ __forceinline__ uint64_t pair_f32(float x, float y) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t z;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(z) : "l"(x), "l"(y));
+  return z;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+  uint64_t z;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(z) : "l"(x), "l"(y));
+  return z;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t w) {
+  uint64_t z;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(z) : "l"(x), "l"(y), "l"(w));
+  return z;
+}
+
+// The codes of eight channels, the first in the low four bits: rint of the correctly rounded quotient
+// (x - lo) / step, which is at most 15 (step is not below span / 15). Adding 1.5 * 2^23 rounds to whole
+// numbers; sums of four codes times powers of 16 are exact in float32. Step 0 or NaN gives zeros.
+__device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float step, float lo, float inverse) {
+  const uint64_t minus_lo = pair_f32(-lo, -lo), minus_step = pair_f32(-step, -step), r = pair_f32(inverse, inverse);
+  const uint64_t whole = pair_f32(12582912.0f, 12582912.0f), back = pair_f32(-12582912.0f, -12582912.0f);
+  uint64_t c[4];  // codes e and e + 4
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint64_t t = add2(pair_f32(x[e], x[e + 4]), minus_lo);
+    const uint64_t q = mul2(t, r);
+    c[e] = add2(add2(fma2(fma2(q, minus_step, t), r, q), whole), back);
+  }
+  const uint64_t sixteen = pair_f32(16.f, 16.f), bits = pair_f32(256.f, 256.f);
+  const uint64_t sum = add2(fma2(fma2(c[3], sixteen, c[2]), bits, fma2(c[1], sixteen, c[0])), pair_f32(8388608.f, 8388608.f));
+  uint32_t w0, w1;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(w0), "=r"(w1) : "l"(sum));
+  return step > 0.f ? __byte_perm(w0, w1, 0x5410) : 0u;
+}
+
+// the values lo + code step of eight codes
+__device__ __forceinline__ void q4_values(uint32_t w, float step, float lo, float (&x)[8]) {
+  const uint64_t steps = pair_f32(step, step), los = pair_f32(lo, lo), back = pair_f32(-8388608.f, -8388608.f);
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {  // 2^23 + code, less 2^23
+    const uint64_t c = add2(pair_f32(__uint_as_float(((w >> (4 * e)) & 15u) | 0x4b000000u),
+                                     __uint_as_float(((w >> (4 * e + 4)) & 15u) | 0x4b000000u)), back);
+    const uint64_t y = fma2(c, steps, los);
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x[e]), "=f"(x[e + 1]) : "l"(y));
+  }
 }
 
 }  // namespace vb

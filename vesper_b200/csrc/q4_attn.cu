@@ -390,27 +390,20 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
 #pragma unroll
     for (int j = 0; j < 8; ++j) tok[j] = tok_c < DK ? to_f32<T>(tokraw[j]) : 0.f;
     float lowest = tok[0], highest = tok[0];
-    bool nan = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lowest = fminf(lowest, tok[j]);
-      highest = fmaxf(highest, tok[j]);
-      nan |= tok[j] != tok[j];
+    for (int j = 1; j < 8; ++j) {
+      lowest = min_nan(lowest, tok[j]);
+      highest = max_nan(highest, tok[j]);
     }
-    if (nan) lowest = highest = __uint_as_float(0x7fc00000u);
 #pragma unroll
     for (int s = 1; s < GS / 8; s <<= 1) {
-      const float l2 = __shfl_xor_sync(0xffffffffu, lowest, s), h2 = __shfl_xor_sync(0xffffffffu, highest, s);
-      const bool bad = lowest != lowest || l2 != l2;
-      lowest = bad ? __uint_as_float(0x7fc00000u) : fminf(lowest, l2);
-      highest = bad ? lowest : fmaxf(highest, h2);
+      lowest = min_nan(lowest, __shfl_xor_sync(0xffffffffu, lowest, s));
+      highest = max_nan(highest, __shfl_xor_sync(0xffffffffu, highest, s));
     }
-    float step, lo;
-    q4_params(lowest, highest, step, lo);
-    const float inverse = step > 0.f ? 1.0f / step : 0.f;
+    float step, lo, inverse;
+    q4_params(lowest, highest, step, lo, inverse);
     tok_params = q4_pack_params(step, lo);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) tok_codes |= q4_code(tok[j], step, lo, inverse) << (4 * j);
+    tok_codes = q4_codes(tok, step, lo, inverse);
     if (tok_c < DK && ht == 0) {
       uint8_t* out = (tok_value ? ring.v_codes : ring.k_codes) + (base + own) * C::CODES;
 #pragma unroll

@@ -1,13 +1,27 @@
 // The 4-bit ring cache: tokens quantised as they are written, and read back at given positions
 // (a RingKVCache, vesper/attention.py:63-139, whose keys and values take five bits a channel).
-// The format is q4.cuh's. One thread per eight channels of a token's key or value: a group's lanes
-// share its extremes by shuffles. HBM bound: 2 bytes in and 0.625 out per bf16 channel.
+// The format is q4.cuh's. A CTA takes some tokens of one (row, key head) (32 at DK 128), keys and values: a thread per
+// eight channels (16 bytes of bf16), a group's extremes by shuffles among its neighbours, and the
+// codes by way of shared memory, where they find their places a byte or a word at a time and leave or arrive in
+// 8-byte pieces of consecutive slots. HBM bound: 2 bytes in and 0.625 out per bf16 channel.
+#include <type_traits>
+
+#include "launch.cuh"
 #include "q4.cuh"
 
 namespace vb {
 namespace {
 
 constexpr int NT = 256;
+
+// how a CTA's threads lie over its tokens: a thread per eight channels, two passes; then a thread per 8 bytes of codes and
+// per group's parameters
+template <int DK>
+struct Layout {
+  static constexpr int PER = DK / 8, RP = NT / PER, ROWS = 2 * RP;  // threads per token, tokens per pass and per CTA
+  static constexpr int GS = q4_group(DK), NG = DK / GS, HALF = DK / 2;
+  static_assert(ROWS * (HALF / 8) <= NT && ROWS * NG <= NT, "one step each");
+};
 
 struct Q4Ring {
   uint8_t* k_codes;
@@ -17,87 +31,225 @@ struct Q4Ring {
   int64_t* pos;
 };
 
-// tokens [B, N] at positions pos; a token is written when its position is not negative and no
-// later token of the chunk takes its slot (positions being consecutive, the one W later)
-template <typename T>
-__global__ void __launch_bounds__(NT) q4_write_kernel(Q4Ring ring, const T* __restrict__ k, int64_t kb, int64_t kt,
-                                                      const T* __restrict__ v, int64_t vb_, int64_t vt,
-                                                      const int64_t* __restrict__ pos, int64_t rows, int N, int HKV,
-                                                      int DK, int W, int SLOTS) {
-  const int per = DK / 8, gs = q4_group(DK), ng = DK / gs;
-  const int64_t id = (int64_t)blockIdx.x * NT + threadIdx.x;
-  const int64_t row = id / per;  // (b, token, head)
-  const int c0 = (int)(id - row * per) * 8;
-  const bool value = blockIdx.y;
-  const bool inside = row < rows;
-  const int64_t token = inside ? row / HKV : 0;
-  const int kh = inside ? (int)(row - token * HKV) : 0;
-  const int64_t b = token / N;
-  const int i = (int)(token - b * N);
-  const int64_t p = inside ? pos[token] : -1;
-  const bool live = p >= 0 && !(i + W < N && pos[token + W] >= 0);
-  float x[8];
-  const T* src = value ? v + b * vb_ + i * vt + (int64_t)kh * DK + c0 : k + b * kb + i * kt + (int64_t)kh * DK + c0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = live ? to_f32<T>(src[e]) : 0.f;
-  float low = x[0], high = x[0];
-  bool nan = false;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    low = fminf(low, x[e]);
-    high = fmaxf(high, x[e]);
-    nan |= x[e] != x[e];
-  }
-  if (nan) low = high = __uint_as_float(0x7fc00000u);
-  // the lanes of a group are neighbours (DK / 8 is a multiple of a group's lanes)
-  for (int o = 1; o < gs / 8; o <<= 1) {
-    const float l2 = __shfl_xor_sync(0xffffffffu, low, o), h2 = __shfl_xor_sync(0xffffffffu, high, o);
-    const bool bad = low != low || l2 != l2;
-    low = bad ? __uint_as_float(0x7fc00000u) : fminf(low, l2);
-    high = bad ? low : fmaxf(high, h2);
-  }
-  if (!live) return;
-  float step, lo;
-  q4_params(low, high, step, lo);
-  const float inverse = step > 0.f ? 1.0f / step : 0.f;
-  const int slot = (int)(p % W);
-  const int64_t at = (b * HKV + kh) * SLOTS + slot;
-  uint8_t* codes = (value ? ring.v_codes : ring.k_codes) + at * (DK / 2);
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const uint32_t byte = q4_code(x[e], step, lo, inverse) | q4_code(x[e + 1], step, lo, inverse) << 4;
-    codes[(value ? q4_value_place(DK, c0 + e) : q4_key_place(DK, c0 + e)) / 2] = (uint8_t)byte;
-  }
-  if (c0 % gs == 0) (value ? ring.v_params : ring.k_params)[at * ng + c0 / gs] = q4_pack_params(step, lo);
-  if (!value && kh == 0 && c0 == 0) ring.pos[b * SLOTS + slot] = p;
+__device__ __forceinline__ int slot_of(int64_t p, int W) {
+  return p < ((int64_t)1 << 32) ? (int)((uint32_t)p % (uint32_t)W) : (int)(p % W);
 }
 
+// eight consecutive elements as they lie in memory; `vec`: on a 16-byte boundary
 template <typename T>
-__global__ void __launch_bounds__(NT) q4_read_kernel(Q4Ring ring, const int64_t* __restrict__ pos, T* __restrict__ k,
-                                                     T* __restrict__ v, uint8_t* __restrict__ held, int64_t rows, int N,
-                                                     int HKV, int DK, int W, int SLOTS) {
-  const int per = DK / 8, gs = q4_group(DK), ng = DK / gs;
-  const int64_t id = (int64_t)blockIdx.x * NT + threadIdx.x;
-  const int64_t row = id / per;
-  if (row >= rows) return;
-  const int c0 = (int)(id - row * per) * 8;
-  const bool value = blockIdx.y;
-  const int64_t token = row / HKV;
-  const int kh = (int)(row - token * HKV);
-  const int64_t b = token / N, p = pos[token];
-  const int slot = p >= 0 ? (int)(p % W) : 0;
-  const bool have = p >= 0 && ring.pos[b * SLOTS + slot] == p;
-  const int64_t at = (b * HKV + kh) * SLOTS + slot;
-  const uint8_t* codes = (value ? ring.v_codes : ring.k_codes) + at * (DK / 2);
-  const uint32_t pr = (value ? ring.v_params : ring.k_params)[at * ng + c0 / gs];
-  T* dst = (value ? v : k) + row * DK + c0;
+struct __align__(16) Raw8 {
+  T v[8];
+  __device__ __forceinline__ void load(const T* __restrict__ p, int vec) {
+    if (vec) {
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const uint32_t byte = codes[(value ? q4_value_place(DK, c0 + e) : q4_key_place(DK, c0 + e)) / 2];
-    dst[e] = from_f32<T>(have ? fmaf((float)(byte & 15u), q4_step(pr), q4_lo(pr)) : 0.f);
-    dst[e + 1] = from_f32<T>(have ? fmaf((float)(byte >> 4), q4_step(pr), q4_lo(pr)) : 0.f);
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = p[e];
+    }
   }
-  if (!value && kh == 0 && c0 == 0) held[token] = have ? 1 : 0;
+};
+
+// the smallest and the largest of eight elements, NaN if one is; 16-bit types two at a time
+__device__ __forceinline__ void extremes(const Raw8<float>& raw, float& low, float& high) {
+  low = high = raw.v[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) {
+    low = min_nan(low, raw.v[e]);
+    high = max_nan(high, raw.v[e]);
+  }
+}
+__device__ __forceinline__ void extremes(const Raw8<__nv_bfloat16>& raw, float& low, float& high) {
+  const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(raw.v);
+  const __nv_bfloat162 l = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
+  const __nv_bfloat162 h = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+  low = min_nan(__low2float(l), __high2float(l));
+  high = max_nan(__low2float(h), __high2float(h));
+}
+__device__ __forceinline__ void extremes(const Raw8<__half>& raw, float& low, float& high) {
+  const __half2* w = reinterpret_cast<const __half2*>(raw.v);
+  const __half2 l = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
+  const __half2 h = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+  low = min_nan(__low2float(l), __high2float(l));
+  high = max_nan(__low2float(h), __high2float(h));
+}
+
+// Tokens [B, N] at positions pos, negative ones (padding, at either end of a row) not written. Of those that share a
+// slot the last is kept: only the last W before a row's padding are looked at.
+template <typename T, int DK>
+__global__ void __launch_bounds__(NT) q4_write_kernel(Q4Ring ring, const T* __restrict__ k, int64_t kb, int64_t kt,
+                                                      const T* __restrict__ v, int64_t vb_, int64_t vt,
+                                                      const int64_t* __restrict__ pos, int vec, int N, int HKV,
+                                                      int W, int SLOTS) {
+  using L = Layout<DK>;
+  constexpr int PER = L::PER, RP = L::RP, ROWS = L::ROWS, GS = L::GS, NG = L::NG, HALF = L::HALF;
+  __shared__ __align__(16) uint8_t codes[2][ROWS][HALF];
+  __shared__ uint32_t params[2][ROWS][NG];
+  __shared__ int slots[ROWS];  // -1: not written
+  // consecutive CTAs take consecutive tokens of a head, whose slots they fill side by side (4 x 32701 tokens, 8 heads of
+  // 128: 170 us; with a token's heads next to each other 186)
+  const int tid = threadIdx.x, blocks = gridDim.x / HKV, kh = blockIdx.x / blocks, block = blockIdx.x - kh * blocks;
+  const int64_t b = blockIdx.y;
+  const int row0 = tid / PER, c0 = tid % PER * 8;
+  const bool busy = RP * PER == NT || tid < RP * PER;
+  grid_wait();
+  grid_release();
+  const int64_t* at = pos + b * N;
+  Raw8<T> raw[2][2];       // [keys, values][pass]
+  int end = N, first = 0;  // the tokens before the padding at the row's end, and the first of this CTA's
+  int64_t p = -1;
+  auto fetch = [&] {  // every load of the thread in flight before any is used
+    first = max(0, end - W) + block * ROWS;
+    if (tid < ROWS && first + tid < end) p = at[first + tid];
+    const T* from[2] = {k + b * kb + (int64_t)(first + row0) * kt + (int64_t)kh * DK + c0,
+                        v + b * vb_ + (int64_t)(first + row0) * vt + (int64_t)kh * DK + c0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (busy && first + row0 + i * RP < end) {
+        raw[0][i].load(from[0] + i * RP * kt, vec);
+        raw[1][i].load(from[1] + i * RP * vt, vec);
+      }
+  };
+  fetch();  // as if there were no padding at the end
+  if (at[N - 1] < 0) {
+    do {  // whole warps look for its beginning, 32 tokens at a time
+      const int i = end - 1 - (tid & 31);
+      const uint32_t found = __ballot_sync(0xffffffffu, i >= 0 && at[i] >= 0);
+      if (found) {
+        end -= __ffs(found) - 1;
+        break;
+      }
+      end -= min(end, 32);
+    } while (end > 0);
+    p = -1;
+    fetch();
+  }
+  if (first >= end) return;
+  if (tid < ROWS) {
+    slots[tid] = p >= 0 ? slot_of(p, W) : -1;
+    if (kh == 0 && p >= 0) ring.pos[b * SLOTS + slots[tid]] = p;
+  }
+#pragma unroll
+  for (int value = 0; value < 2; ++value)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // a token that is not written holds what it may here and is left out below
+      const int row = row0 + i * RP;
+      float x[8], low, high;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = to_f32<T>(raw[value][i].v[e]);
+      extremes(raw[value][i], low, high);
+      // the lanes of a group are neighbours (PER is a multiple of a group's lanes)
+#pragma unroll
+      for (int o = 1; o < GS / 8; o <<= 1) {
+        low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
+      }
+      float step, lo, inverse;
+      q4_params(low, high, step, lo, inverse);
+      const uint32_t w = q4_codes(x, step, lo, inverse);
+      if (!busy) continue;
+      uint8_t* to = codes[value][row];
+      if (value) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[q4_value_place(DK, c0 + 2 * e) / 2] = (uint8_t)(w >> (8 * e));
+      } else if constexpr (GS == 32) {
+        *reinterpret_cast<uint32_t*>(to + q4_key_place(DK, c0) / 2) = w;
+      } else {
+        *reinterpret_cast<uint16_t*>(to + q4_key_place(DK, c0) / 2) = (uint16_t)w;
+        *reinterpret_cast<uint16_t*>(to + q4_key_place(DK, c0 + 4) / 2) = (uint16_t)(w >> 16);
+      }
+      if (c0 % GS == 0) params[value][row][c0 / GS] = q4_pack_params(step, lo);
+    }
+  __syncthreads();
+  const int64_t base = (b * HKV + kh) * SLOTS;
+  {
+    const int row = tid / (HALF / 8), c = tid % (HALF / 8);
+    if (row < ROWS && slots[row] >= 0) {
+      const int64_t to = (base + slots[row]) * (HALF / 8) + c;
+      reinterpret_cast<uint2*>(ring.k_codes)[to] = reinterpret_cast<const uint2*>(codes[0][row])[c];
+      reinterpret_cast<uint2*>(ring.v_codes)[to] = reinterpret_cast<const uint2*>(codes[1][row])[c];
+    }
+  }
+  const int row = tid / NG, g = tid % NG;
+  if (row < ROWS && slots[row] >= 0) {
+    const int64_t to = (base + slots[row]) * NG + g;
+    ring.k_params[to] = params[0][row][g];
+    ring.v_params[to] = params[1][row][g];
+  }
+}
+
+template <typename T, int DK>
+__global__ void __launch_bounds__(NT) q4_read_kernel(Q4Ring ring, const int64_t* __restrict__ pos, T* __restrict__ k,
+                                                     T* __restrict__ v, uint8_t* __restrict__ held, int N, int HKV,
+                                                     int W, int SLOTS) {
+  using L = Layout<DK>;
+  constexpr int PER = L::PER, RP = L::RP, ROWS = L::ROWS, GS = L::GS, NG = L::NG, HALF = L::HALF;
+  __shared__ __align__(16) uint8_t codes[2][ROWS][HALF];
+  __shared__ uint32_t params[2][ROWS][NG];
+  __shared__ int slots[ROWS];  // -1: no position that a ring could hold
+  __shared__ bool have[ROWS];
+  // consecutive CTAs take the heads of the same tokens, whose values lie side by side (the same: 151 us; by head 157)
+  const int tid = threadIdx.x, block = blockIdx.x / HKV, kh = blockIdx.x - block * HKV, first = block * ROWS;
+  const int64_t b = blockIdx.y;
+  grid_wait();
+  grid_release();
+  const int64_t p = tid < ROWS && first + tid < N ? pos[b * N + first + tid] : -1;
+  if (tid < ROWS) slots[tid] = p >= 0 ? slot_of(p, W) : -1;
+  __syncthreads();
+  const int64_t base = (b * HKV + kh) * SLOTS;
+  // the slot is read before it is known to hold the position
+  if (tid < ROWS) {
+    have[tid] = p >= 0 && ring.pos[b * SLOTS + slots[tid]] == p;
+    if (kh == 0 && first + tid < N) held[b * N + first + tid] = have[tid];
+  }
+  {
+    const int row = tid / (HALF / 8), c = tid % (HALF / 8);
+    if (row < ROWS && slots[row] >= 0) {
+      const int64_t from = (base + slots[row]) * (HALF / 8) + c;
+      reinterpret_cast<uint2*>(codes[0][row])[c] = reinterpret_cast<const uint2*>(ring.k_codes)[from];
+      reinterpret_cast<uint2*>(codes[1][row])[c] = reinterpret_cast<const uint2*>(ring.v_codes)[from];
+    }
+  }
+  {
+    const int row = tid / NG, g = tid % NG;
+    if (row < ROWS && slots[row] >= 0) {
+      const int64_t from = (base + slots[row]) * NG + g;
+      params[0][row][g] = ring.k_params[from];
+      params[1][row][g] = ring.v_params[from];
+    }
+  }
+  __syncthreads();
+  const int row0 = tid / PER, c0 = tid % PER * 8;
+  if (RP * PER < NT && tid >= RP * PER) return;
+#pragma unroll
+  for (int value = 0; value < 2; ++value)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = row0 + i * RP;
+      if (first + row >= N) continue;
+      float x[8];
+      if (have[row]) {
+        const uint8_t* from = codes[value][row];
+        uint32_t w = 0;
+        if (value) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w |= (uint32_t)from[q4_value_place(DK, c0 + 2 * e) / 2] << (8 * e);
+        } else if constexpr (GS == 32) {
+          w = *reinterpret_cast<const uint32_t*>(from + q4_key_place(DK, c0) / 2);
+        } else {
+          w = *reinterpret_cast<const uint16_t*>(from + q4_key_place(DK, c0) / 2) |
+              (uint32_t)*reinterpret_cast<const uint16_t*>(from + q4_key_place(DK, c0 + 4) / 2) << 16;
+        }
+        const uint32_t pr = params[value][row][c0 / GS];
+        q4_values(w, q4_step(pr), q4_lo(pr), x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+      }
+      store_vec<T, 8>((value ? v : k) + ((b * N + first + row) * HKV + kh) * DK + c0, x);
+    }
 }
 
 int check_ring(const char* what, int B, int N, int HKV, int DK, int W, int SLOTS, int dtype) {
@@ -107,9 +259,24 @@ int check_ring(const char* what, int B, int N, int HKV, int DK, int W, int SLOTS
   VB_REQUIRE(SLOTS % Q4_TILE == 0 && SLOTS >= W, "%s: %d slots must be a multiple of %d holding the window %d", what,
              SLOTS, Q4_TILE, W);
   VB_REQUIRE(dtype_size(dtype) > 0, "%s: unsupported dtype code %d", what, dtype);
-  const int64_t blocks = ((int64_t)B * N * HKV * (DK / 8) + NT - 1) / NT;
-  VB_REQUIRE(blocks < (int64_t(1) << 31), "%s: %d x %d tokens exceed the grid", what, B, N);
+  VB_REQUIRE(B <= 65535 && (int64_t)N * HKV < (int64_t(1) << 31), "%s: %d rows of %d tokens x %d key heads exceed the grid",
+             what, B, N, HKV);
   return VB_OK;
+}
+
+// runs f with DK as a compile-time constant
+template <typename F>
+int with_head_dim(int DK, F f) {
+  switch (DK) {
+    case 16: return f(std::integral_constant<int, 16>{});
+    case 32: return f(std::integral_constant<int, 32>{});
+    case 48: return f(std::integral_constant<int, 48>{});
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 80: return f(std::integral_constant<int, 80>{});
+    case 96: return f(std::integral_constant<int, 96>{});
+    case 112: return f(std::integral_constant<int, 112>{});
+    default: return f(std::integral_constant<int, 128>{});
+  }
 }
 
 }  // namespace
@@ -126,13 +293,17 @@ extern "C" int vb_q4_write(void* k_codes, void* k_params, void* v_codes, void* v
   if (B == 0 || N == 0) return VB_OK;
   VB_REQUIRE(k_codes && k_params && v_codes && v_params && ring_pos && k && v && pos, "q4_write: null pointer");
   const Q4Ring ring{(uint8_t*)k_codes, (uint32_t*)k_params, (uint8_t*)v_codes, (uint32_t*)v_params, ring_pos};
-  const int64_t rows = (int64_t)B * N * HKV;
-  const dim3 grid((unsigned)((rows * (DK / 8) + NT - 1) / NT), 2);
+  VB_REQUIRE(aligned16(k_codes) && aligned16(k_params) && aligned16(v_codes) && aligned16(v_params),
+             "q4_write: the ring's buffers must start on 16-byte boundaries");
+  const int size = dtype_size(dtype);
+  const int vec = aligned16(k) && aligned16(v) && k_batch * size % 16 == 0 && k_token * size % 16 == 0 &&
+                  v_batch * size % 16 == 0 && v_token * size % 16 == 0;
   return VB_DISPATCH_DTYPE(dtype, T, [&]() -> int {
-    q4_write_kernel<T><<<grid, NT, 0, (cudaStream_t)stream>>>(ring, (const T*)k, k_batch, k_token, (const T*)v, v_batch,
-                                                              v_token, pos, rows, N, HKV, DK, W, SLOTS);
-    VB_LAUNCH_CHECK("q4_write");
-    return VB_OK;
+    return with_head_dim(DK, [&](auto dk) -> int {
+      return launch_early("q4_write", q4_write_kernel<T, decltype(dk)::value>, dim3((min(N, W) + Layout<decltype(dk)::value>::ROWS - 1) / Layout<decltype(dk)::value>::ROWS * HKV, B), NT,
+                          0, 1, (cudaStream_t)stream, ring, (const T*)k, k_batch, k_token, (const T*)v, v_batch, v_token, pos,
+                          vec, N, HKV, W, SLOTS);
+    });
   });
 }
 
@@ -144,11 +315,13 @@ extern "C" int vb_q4_read(const void* k_codes, const void* k_params, const void*
   if (B == 0 || N == 0) return VB_OK;
   VB_REQUIRE(k_codes && k_params && v_codes && v_params && ring_pos && pos && k && v && held, "q4_read: null pointer");
   const Q4Ring ring{(uint8_t*)k_codes, (uint32_t*)k_params, (uint8_t*)v_codes, (uint32_t*)v_params, (int64_t*)ring_pos};
-  const int64_t rows = (int64_t)B * N * HKV;
-  const dim3 grid((unsigned)((rows * (DK / 8) + NT - 1) / NT), 2);
+  VB_REQUIRE(aligned16(k_codes) && aligned16(k_params) && aligned16(v_codes) && aligned16(v_params) && aligned16(k) &&
+                 aligned16(v),
+             "q4_read: the buffers must start on 16-byte boundaries");
   return VB_DISPATCH_DTYPE(dtype, T, [&]() -> int {
-    q4_read_kernel<T><<<grid, NT, 0, (cudaStream_t)stream>>>(ring, pos, (T*)k, (T*)v, held, rows, N, HKV, DK, W, SLOTS);
-    VB_LAUNCH_CHECK("q4_read");
-    return VB_OK;
+    return with_head_dim(DK, [&](auto dk) -> int {
+      return launch_early("q4_read", q4_read_kernel<T, decltype(dk)::value>, dim3((N + Layout<decltype(dk)::value>::ROWS - 1) / Layout<decltype(dk)::value>::ROWS * HKV, B), NT, 0, 1,
+                          (cudaStream_t)stream, ring, pos, (T*)k, (T*)v, held, N, HKV, W, SLOTS);
+    });
   });
 }
