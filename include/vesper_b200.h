@@ -420,7 +420,7 @@ VB_API int vb_linear_q8(const int8_t *xq, int64_t ldx, const float *xs, const in
  * [B, HKV, DK] (row strides in elements), pos [B]: the token is written and attends the slots with
  * p - W < pos <= p, itself included, as the ring holds them (scale 1/sqrt(DK), head h reading key
  * head h / (H / HKV)); o [B, H, DK], zero in a row whose position is negative (which writes nothing).
- * `workspace`: vb_q4_attend_workspace bytes, 16-byte aligned. */
+ * `workspace`: vb_q4_attend_workspace bytes, 16-byte aligned (0: none, it may be NULL). */
 VB_API int vb_q4_write(void *k_codes, void *k_params, void *v_codes, void *v_params,
                        int64_t *ring_pos, const void *k, int64_t k_batch, int64_t k_token,
                        const void *v, int64_t v_batch, int64_t v_token, const int64_t *pos, int B,

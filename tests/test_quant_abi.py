@@ -39,4 +39,5 @@ def test_the_4_bit_cache_entry_points_refuse_bad_arguments_without_a_gpu() -> No
     attend = [None, 0, None, 0, None, 0, None, *ring, None, None]
     _refused("vb_q4_attend", *attend, 1, 3, 2, 64, 64, 64, 0, None, match="not a multiple of 2 key heads")
     _refused("vb_q4_attend", *attend, 1, 2, 2, 64, 64, 64, 0, None, match="null pointer")
-    assert _lib.query("vb_q4_attend_workspace", 1, 8, 2, 64, 4096) >= 16
+    assert _lib.query("vb_q4_attend_workspace", 64, 8, 2, 64, 512) == 0  # a CTA per row and key head
+    assert _lib.query("vb_q4_attend_workspace", 1, 8, 2, 64, 4096) > 0

@@ -135,7 +135,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream(device: torch.device) -> int:
     """torch's current CUDA stream on ``device`` as a raw handle."""
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

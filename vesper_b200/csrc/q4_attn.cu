@@ -778,9 +778,9 @@ int head_tiles_of(int H, int HKV) { return (H / HKV + HEADS - 1) / HEADS; }
 using namespace vb;
 
 extern "C" size_t vb_q4_attend_workspace(int B, int H, int HKV, int DK, int W) {
-  if (B <= 0 || H <= 0 || HKV <= 0 || H % HKV || DK <= 0 || W <= 0) return 16;
+  if (B <= 0 || H <= 0 || HKV <= 0 || H % HKV || DK <= 0 || W <= 0) return 0;
   const int units = HKV * head_tiles_of(H, HKV), ctas = shared_ctas(B, units, DK, W);
-  if (ctas == 0) return 16;
+  if (ctas == 0) return 0;
   return sizeof(int2) * (size_t)B * units + sizeof(float) * 2 * (size_t)ctas * HEADS * (DK + 2);
 }
 
@@ -795,12 +795,14 @@ extern "C" int vb_q4_attend(const void* q, int64_t q_row, const void* k_new, int
              SLOTS, Q4_TILE, W);
   VB_REQUIRE(dtype_size(dtype) > 0, "q4_attend: unsupported dtype code %d", dtype);
   if (B == 0) return VB_OK;
-  VB_REQUIRE(q && k_new && v_new && pos && k_codes && k_params && v_codes && v_params && ring_pos && o && workspace,
+  VB_REQUIRE(q && k_new && v_new && pos && k_codes && k_params && v_codes && v_params && ring_pos && o,
              "q4_attend: null pointer");
   VB_REQUIRE(aligned16(k_codes) && aligned16(k_params) && aligned16(v_codes) && aligned16(v_params) && aligned16(ring_pos),
              "q4_attend: the ring's buffers must start on 16-byte boundaries");
-  VB_REQUIRE(aligned16(workspace), "q4_attend: the workspace must start on a 16-byte boundary");
+
   const int head_tiles = head_tiles_of(H, HKV), units = HKV * head_tiles, ctas = shared_ctas(B, units, DK, W);
+  VB_REQUIRE(ctas == 0 || (workspace != nullptr && aligned16(workspace)),
+             "q4_attend: a workspace of vb_q4_attend_workspace bytes must start on a 16-byte boundary");
   VB_REQUIRE(B <= 65535 && units <= 65535, "q4_attend: %d rows of %d head tiles exceed the grid", B, units);
   const Ring ring{(uint8_t*)k_codes, (uint32_t*)k_params, (uint8_t*)v_codes, (uint32_t*)v_params, ring_pos};
   const float scale_log2 = 1.4426950408889634f / sqrtf((float)DK);

@@ -22,6 +22,7 @@ only through torch and can be captured in a CUDA graph.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 from torch import Tensor
@@ -82,7 +83,27 @@ def q4_ring_empty(b: int, hkv: int, dk: int, window: int, device: torch.device) 
 
 
 def _check_ring(ring: Q4RingKVCache, what: str) -> tuple[int, int, int, int]:
-    """``(b, hkv, dk, slots)`` of a well-formed ring on CUDA."""
+    """``(b, hkv, dk, slots)`` of a well-formed ring on CUDA: accepts in one expression what is
+    well-formed, else finds out what is not."""
+    kc, kp, vc, vp, pos = ring.k_codes, ring.k_params, ring.v_codes, ring.v_params, ring.pos
+    if kc.dim() == 4:
+        shape, device = kc.shape, kc.device
+        b, hkv, slots, half = shape
+        params = (b, hkv, slots, half // 16 if half % 16 == 0 else half // 8, 2)
+        if (
+            half % 8 == 0 and 8 <= half <= MAX_HEAD_DIM // 2 and slots % SLOT_TILE == 0 and slots >= ring.window >= 1
+            and vc.shape == shape and kp.shape == params and vp.shape == params and pos.shape == (b, slots)
+            and kc.dtype == torch.uint8 == vc.dtype and kp.dtype == torch.bfloat16 == vp.dtype and pos.dtype == torch.int64
+            and kc.is_cuda and kp.device == device and vc.device == device and vp.device == device and pos.device == device
+            and kc.is_contiguous() and kp.is_contiguous() and vc.is_contiguous() and vp.is_contiguous()
+            and pos.is_contiguous()
+            and (kc.data_ptr() | kp.data_ptr() | vc.data_ptr() | vp.data_ptr() | pos.data_ptr()) % 16 == 0
+        ):  # fmt: skip
+            return b, hkv, 2 * half, slots
+    return _explain_ring(ring, what)
+
+
+def _explain_ring(ring: Q4RingKVCache, what: str) -> tuple[int, int, int, int]:
     dims: Dims = {}
     check_shape("ring.k_codes", ring.k_codes, ("b", "hkv", "slots", "half"), dims, torch.uint8)
     b, hkv, slots, dk = dims["b"], dims["hkv"], dims["slots"], 2 * dims["half"]
@@ -119,16 +140,28 @@ def _ring_ptrs(ring: Q4RingKVCache) -> tuple[int, int, int, int, int]:
 
 def _check_tokens(ring: Q4RingKVCache, k: Tensor, v: Tensor, pos: Tensor, what: str) -> tuple[int, int, int, int, int]:
     b, hkv, dk, slots = _check_ring(ring, what)
-    dims: Dims = {"b": b, "hkv": hkv, "dk": dk}
-    check_shape("k", k, ("b", "n", "hkv", "dk"), dims)
-    check_shape("v", v, ("b", "n", "hkv", "dk"), dims)
-    check_shape("pos", pos, ("b", "n"), dims, torch.long)
-    if k.dtype not in SUPPORTED or v.dtype != k.dtype:
-        msg = f"k, v: one dtype of {SUPPORTED}, got {k.dtype} and {v.dtype}"
-        raise ContractError(msg)
-    require_cuda(what, ring.pos, k=k, v=v, positions=pos)
+    device = ring.pos.device
+    if not (
+        k.dim() == 4 and k.shape[0] == b and k.shape[2] == hkv and k.shape[3] == dk and v.shape == k.shape
+        and pos.shape == k.shape[:2] and pos.dtype == torch.int64 and k.dtype in SUPPORTED and v.dtype == k.dtype
+        and k.device == device and v.device == device and pos.device == device
+    ):  # fmt: skip
+        dims: Dims = {"b": b, "hkv": hkv, "dk": dk}
+        check_shape("k", k, ("b", "n", "hkv", "dk"), dims)
+        check_shape("v", v, ("b", "n", "hkv", "dk"), dims)
+        check_shape("pos", pos, ("b", "n"), dims, torch.long)
+        if k.dtype not in SUPPORTED or v.dtype != k.dtype:
+            msg = f"k, v: one dtype of {SUPPORTED}, got {k.dtype} and {v.dtype}"
+            raise ContractError(msg)
+        require_cuda(what, ring.pos, k=k, v=v, positions=pos)
     serving_only(what, k, v)
-    return b, dims["n"], hkv, dk, slots
+    return b, k.shape[1], hkv, dk, slots
+
+
+@lru_cache(maxsize=256)
+def _attend_workspace(b: int, heads: int, hkv: int, dk: int, window: int) -> int:
+    """The library's answer for these sizes (0: none needed)."""
+    return _lib.query("vb_q4_attend_workspace", b, heads, hkv, dk, window)
 
 
 def q4_write_(ring: Q4RingKVCache, k: Tensor, v: Tensor, pos: Tensor) -> Q4RingKVCache:
@@ -194,27 +227,30 @@ def q4_attend_(q: Tensor, k: Tensor, v: Tensor, pos: Tensor, ring: Q4RingKVCache
     """
     b, n, hkv, dk, slots = _check_tokens(ring, k, v, pos, "4-bit ring attention")
     dims: Dims = {"b": b, "one": 1, "dk": dk}
-    check_shape("q", q, ("b", "one", "h", "dk"), dims)
+    if not (q.dim() == 4 and q.shape[0] == b and q.shape[1] == 1 and q.shape[3] == dk):
+        check_shape("q", q, ("b", "one", "h", "dk"), dims)
     if n != 1:
         msg = f"k: axis 1 must be 1, got {n} (one token per row)"
         raise ContractError(msg)
-    heads = dims["h"]
+    heads = q.shape[2]
     if heads < 1 or heads % hkv != 0:
         msg = f"{heads} query heads are not a multiple of {hkv} key heads"
         raise ContractError(msg)
     if q.dtype != k.dtype:
         msg = f"k: dtype must be {q.dtype} (q's), got {k.dtype}"
         raise ContractError(msg)
-    require_cuda("4-bit ring attention", ring.pos, q=q)
+    if q.device != k.device:
+        require_cuda("4-bit ring attention", ring.pos, q=q)
     serving_only("4-bit ring attention", q)
     o = torch.empty(b, 1, heads, dk, dtype=q.dtype, device=q.device)
     if b == 0:
         return o
     q, k, v, pos = _tokens(q), _tokens(k), _tokens(v), pos.contiguous()
-    ws = _lib.workspace(_lib.query("vb_q4_attend_workspace", b, heads, hkv, dk, ring.window), q.device)
+    nbytes = _attend_workspace(b, heads, hkv, dk, ring.window)
+    ws = _lib.workspace(nbytes, q.device) if nbytes else None
     _lib.call(
         "vb_q4_attend", q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-        pos.data_ptr(), *_ring_ptrs(ring), o.data_ptr(), ws.data_ptr(), b, heads, hkv, dk, ring.window, slots,
+        pos.data_ptr(), *_ring_ptrs(ring), o.data_ptr(), _lib.ptr(ws), b, heads, hkv, dk, ring.window, slots,
         _lib.DTYPE_CODE[q.dtype], _lib.stream(q.device),
     )  # fmt: skip
     return o

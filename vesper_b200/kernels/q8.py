@@ -32,24 +32,35 @@ SUPPORTED = (torch.float32, torch.bfloat16, torch.float16)
 MAX_K = 131056  # largest inner dimension whose int8 sums stay in int32
 
 
-def serving_only(what: str, *tensors: Tensor | None) -> None:
+def serving_only(what: str, *tensors: Tensor) -> None:
     """Refuse inputs that autograd is recording: these operators have no gradient."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        msg = f"the {what} has no gradient: call it under torch.no_grad()"
-        raise ContractError(msg)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                msg = f"the {what} has no gradient: call it under torch.no_grad()"
+                raise ContractError(msg)
 
 
 def _codes(x: Tensor) -> tuple[Tensor, Tensor, int]:
     """Empty codes and scales for ``x``'s rows, and the codes' row pitch."""
-    width = x.shape[-1]
+    lead, width, device = x.shape[:-1], x.shape[-1], x.device
+    scale = torch.empty(lead, dtype=torch.float32, device=device)
+    if width % 16 == 0:
+        return torch.empty(x.shape, dtype=torch.int8, device=device), scale, width
     pitch = -(-width // 16) * 16
-    q = torch.empty(*x.shape[:-1], pitch, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    return (q if pitch == width else q[..., :width]), scale, pitch
+    return torch.empty(*lead, pitch, dtype=torch.int8, device=device)[..., :width], scale, pitch
 
 
-def _check_norm(x: Tensor, weight: Tensor, what: str) -> None:
-    require_cuda(what, x, weight=weight)
+def _check_norm(x: Tensor, r: Tensor | None, weight: Tensor) -> None:
+    """Accepts in one expression what is well-formed, else finds out what is not."""
+    device = x.device
+    if (
+        x.is_cuda and x.dtype in SUPPORTED and x.dim() >= 1 and weight.dim() == 1 and x.shape[-1] == weight.shape[0] >= 1
+        and weight.device == device
+        and (r is None or (x.dtype == torch.float32 and r.shape == x.shape and r.dtype in SUPPORTED and r.device == device))
+    ):  # fmt: skip
+        return
+    require_cuda("8-bit RMSNorm", x, weight=weight, r=r)
     if x.dtype not in SUPPORTED:
         msg = f"x: dtype must be one of {SUPPORTED}, got {x.dtype}"
         raise ContractError(msg)
@@ -59,19 +70,36 @@ def _check_norm(x: Tensor, weight: Tensor, what: str) -> None:
     if weight.shape != (x.shape[-1],):
         msg = f"weight: expected shape ({x.shape[-1]},), got {tuple(weight.shape)}"
         raise ContractError(msg)
+    assert r is not None
+    if x.dtype != torch.float32:
+        msg = f"x: dtype must be {torch.float32} (the residual stream), got {x.dtype}"
+        raise ContractError(msg)
+    if r.shape != x.shape:
+        msg = f"r: expected shape {tuple(x.shape)}, got {tuple(r.shape)}"
+        raise ContractError(msg)
+    msg = f"r: dtype must be one of {SUPPORTED}, got {r.dtype}"
+    raise ContractError(msg)
 
 
 def _norm(x: Tensor, r: Tensor | None, weight: Tensor, floor: float, eps: float):
-    serving_only("8-bit RMSNorm", x, r, weight)
-    width = x.shape[-1]
+    _check_norm(x, r, weight)
+    width = weight.shape[0]
     x = x.contiguous()
-    w32 = weight.to(torch.float32).contiguous()
+    if weight.dtype != torch.float32 or not weight.is_contiguous():
+        weight = weight.to(torch.float32).contiguous()
     q, scale, pitch = _codes(x)
-    total = None if r is None else torch.empty_like(x)
+    code = _lib.DTYPE_CODE
+    if r is None:
+        serving_only("8-bit RMSNorm", x, weight)
+        total, total_ptr, r_ptr, r_code = None, None, None, 0
+    else:
+        serving_only("8-bit RMSNorm", x, r, weight)
+        r = r.contiguous()
+        total = torch.empty_like(x)
+        total_ptr, r_ptr, r_code = total.data_ptr(), r.data_ptr(), code[r.dtype]
     _lib.call(
-        "vb_rms_norm_q8", x.data_ptr(), _lib.ptr(r), w32.data_ptr(), _lib.ptr(total), q.data_ptr(), pitch,
-        scale.data_ptr(), x.numel() // width, width, floor, eps, _lib.DTYPE_CODE[x.dtype],
-        _lib.DTYPE_CODE[x.dtype if r is None else r.dtype], _lib.stream(x.device),
+        "vb_rms_norm_q8", x.data_ptr(), r_ptr, weight.data_ptr(), total_ptr, q.data_ptr(), pitch, scale.data_ptr(),
+        x.numel() // width, width, floor, eps, code[x.dtype], r_code, _lib.stream(x.device),
     )  # fmt: skip
     return total, q, scale
 
@@ -84,7 +112,6 @@ def rms_norm_q8(x: Tensor, weight: Tensor, floor: float, eps: float) -> tuple[Te
     Raises:
         ContractError: on a CPU tensor, an unsupported dtype or a weight of another width.
     """
-    _check_norm(x, weight, "8-bit RMSNorm")
     _, q, scale = _norm(x, None, weight, floor, eps)
     return q, scale
 
@@ -98,18 +125,7 @@ def add_rms_norm_q8(x: Tensor, r: Tensor, weight: Tensor, floor: float, eps: flo
     Raises:
         ContractError: as ``rms_norm_q8``, or where ``x`` is not float32 or ``r`` has another shape.
     """
-    _check_norm(x, weight, "8-bit RMSNorm")
-    require_cuda("8-bit RMSNorm", x, r=r)
-    if x.dtype != torch.float32:
-        msg = f"x: dtype must be {torch.float32} (the residual stream), got {x.dtype}"
-        raise ContractError(msg)
-    if r.shape != x.shape:
-        msg = f"r: expected shape {tuple(x.shape)}, got {tuple(r.shape)}"
-        raise ContractError(msg)
-    if r.dtype not in SUPPORTED:
-        msg = f"r: dtype must be one of {SUPPORTED}, got {r.dtype}"
-        raise ContractError(msg)
-    return _norm(x, r.contiguous(), weight, floor, eps)
+    return _norm(x, r, weight, floor, eps)
 
 
 def quantize_rows_q8(x: Tensor, *, relu_square: bool = False) -> tuple[Tensor, Tensor]:
@@ -161,27 +177,60 @@ def dequantize_rows_q8(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.floa
         ContractError: on a CPU tensor, codes that are not int8, scales that are not float32 of the
             rows' shape or an unsupported ``dtype``.
     """
-    require_cuda("8-bit rows", q, scale=scale)
-    if q.dtype != torch.int8 or scale.dtype != torch.float32:
-        msg = f"q, scale: dtypes must be {torch.int8} and {torch.float32}, got {q.dtype} and {scale.dtype}"
-        raise ContractError(msg)
-    if q.dim() < 1 or q.shape[:-1] != scale.shape or q.shape[-1] < 1:
+    if not (
+        q.is_cuda and scale.device == q.device and q.dtype == torch.int8 and scale.dtype == torch.float32 and q.dim() >= 1
+        and q.shape[-1] >= 1 and scale.shape == q.shape[:-1] and dtype in SUPPORTED
+    ):  # fmt: skip
+        require_cuda("8-bit rows", q, scale=scale)
+        if q.dtype != torch.int8 or scale.dtype != torch.float32:
+            msg = f"q, scale: dtypes must be {torch.int8} and {torch.float32}, got {q.dtype} and {scale.dtype}"
+            raise ContractError(msg)
+        if dtype not in SUPPORTED:
+            msg = f"dtype: must be one of {SUPPORTED}, got {dtype}"
+            raise ContractError(msg)
         msg = f"scale: expected one per row of q {tuple(q.shape)}, got shape {tuple(scale.shape)}"
-        raise ContractError(msg)
-    if dtype not in SUPPORTED:
-        msg = f"dtype: must be one of {SUPPORTED}, got {dtype}"
         raise ContractError(msg)
     width = q.shape[-1]
     rows = q.numel() // width
-    flat = q.reshape(rows, width)  # a view of codes as this module lays them out
-    if (width > 1 and flat.stride(1) != 1) or (rows > 1 and flat.stride(0) < width):
-        flat = flat.contiguous()
+    if q.is_contiguous():
+        flat, pitch = q, width
+    else:
+        flat = q.reshape(rows, width)  # a view of codes as this module lays them out
+        if (width > 1 and flat.stride(1) != 1) or (rows > 1 and flat.stride(0) < width):
+            flat = flat.contiguous()
+        pitch = flat.stride(0) if rows > 1 else width
     y = torch.empty(q.shape, dtype=dtype, device=q.device)
     _lib.call(
-        "vb_dequantize_rows_q8", flat.data_ptr(), flat.stride(0) if rows > 1 else width,
-        scale.contiguous().data_ptr(), y.data_ptr(), rows, width, _lib.DTYPE_CODE[dtype], _lib.stream(q.device),
+        "vb_dequantize_rows_q8", flat.data_ptr(), pitch, scale.contiguous().data_ptr(), y.data_ptr(), rows, width, _lib.DTYPE_CODE[dtype], _lib.stream(q.device),
     )  # fmt: skip
     return y
+
+
+def _check_linear(xq: Tensor, xs: Tensor, wq: Tensor, ws: Tensor, out_dtype: torch.dtype) -> tuple[int, int]:
+    """``(N, K)``: accepts in one expression what is well-formed, else finds out what is not."""
+    device = xq.device
+    if (
+        wq.dim() == 2 and xq.dim() >= 1 and wq.dtype == torch.int8 == xq.dtype and xs.dtype == torch.float32 == ws.dtype
+        and 1 <= wq.shape[1] <= MAX_K and xq.shape[-1] == wq.shape[1] and xs.shape == xq.shape[:-1]
+        and ws.shape == wq.shape[:1] and wq.shape[0] >= 1 and out_dtype in SUPPORTED and xq.is_cuda
+        and xs.device == device and wq.device == device and ws.device == device
+    ):  # fmt: skip
+        return wq.shape[0], wq.shape[1]
+    dims: Dims = {}
+    check_shape("wq", wq, ("N", "K"), dims, torch.int8)
+    check_shape("ws", ws, ("N",), dims, torch.float32)
+    if xq.dim() < 1 or xq.dtype != torch.int8 or xq.shape[-1] != dims["K"]:
+        msg = f"xq: expected int8 rows of {dims['K']} channels, got {xq.dtype} {tuple(xq.shape)}"
+        raise ContractError(msg)
+    if xs.shape != xq.shape[:-1] or xs.dtype != torch.float32:
+        msg = f"xs: expected one float32 scale per row of xq {tuple(xq.shape)}, got {xs.dtype} {tuple(xs.shape)}"
+        raise ContractError(msg)
+    if out_dtype not in SUPPORTED:
+        msg = f"out_dtype: must be one of {SUPPORTED}, got {out_dtype}"
+        raise ContractError(msg)
+    require_cuda("int8 product", xq, xs=xs, wq=wq, ws=ws)
+    msg = f"wq: expected at least one row of 1 to {MAX_K} channels, got shape {tuple(wq.shape)}"
+    raise ContractError(msg)
 
 
 def linear_q8(xq: Tensor, xs: Tensor, wq: Tensor, ws: Tensor, out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
@@ -196,23 +245,7 @@ def linear_q8(xq: Tensor, xs: Tensor, wq: Tensor, ws: Tensor, out_dtype: torch.d
         ContractError: on a shape or dtype mismatch, a CPU tensor or ``K`` above 131056 (where a sum
             of int8 products may leave int32).
     """
-    dims: Dims = {}
-    check_shape("wq", wq, ("N", "K"), dims, torch.int8)
-    check_shape("ws", ws, ("N",), dims, torch.float32)
-    if xq.dim() < 1 or xq.dtype != torch.int8 or xq.shape[-1] != dims["K"]:
-        msg = f"xq: expected int8 rows of {dims['K']} channels, got {xq.dtype} {tuple(xq.shape)}"
-        raise ContractError(msg)
-    if xs.shape != xq.shape[:-1] or xs.dtype != torch.float32:
-        msg = f"xs: expected one float32 scale per row of xq {tuple(xq.shape)}, got {xs.dtype} {tuple(xs.shape)}"
-        raise ContractError(msg)
-    if out_dtype not in SUPPORTED:
-        msg = f"out_dtype: must be one of {SUPPORTED}, got {out_dtype}"
-        raise ContractError(msg)
-    require_cuda("int8 product", xq, xs=xs, wq=wq, ws=ws)
-    n, k = dims["N"], dims["K"]
-    if n < 1 or not 1 <= k <= MAX_K:
-        msg = f"wq: expected at least one row of 1 to {MAX_K} channels, got shape {tuple(wq.shape)}"
-        raise ContractError(msg)
+    n, k = _check_linear(xq, xs, wq, ws, out_dtype)
     flat = xq if xq.dim() == 2 else xq.reshape(-1, k)
     rows, ldx = _pitched(flat)
     weights, ldw = _pitched(wq)
