@@ -9,18 +9,18 @@
 //   scores  S[slot, head] = sum_g step[slot, g] (sum_{c in g} code q) + lo[slot, g] (sum_{c in g} q):
 //     m16n8k16 in f16, slots as rows. A code in the low four bits of a half is the subnormal code 2^-24, one
 //     in the next four bits 16 code 2^-24, both exact, so a word of eight codes needs one shift and
-//     four ANDs; the queries are scaled per head by a power of two to fit f16 (an f32 query takes two terms) and
+//     four ANDs; the queries are scaled per head by a power of two to fit f16 and
 //     divided by 16 where their codes come 16-fold. The group's step and lo are applied to the float32 sums.
 //   output  O[channel, head] = sum_slot (w step) code + w lo: m16n8k16 in f16, channels as rows, the codes again as
 //     they are (those in the upper four bits make their rows of O 16-fold, taken off at the end). The products w step
 //     are rounded to f16 (2^-12 of each, of both signs), whose range they fit because the scores' reference is chosen
-//     with the largest step in view. They cross from the scores' layout to the operand's by movmatrix. For float32
-//     they are held in three bf16 terms and the codes as bf16 code - 8, one OR and one subtraction per pair: sums of
-//     numbers around zero, which the matrix unit's float32 sums keep to 1e-6 of the output.
-// A reference r and the sum of the weights 2^(score - r) per warp and head in float32; r rises only when a weight times
-// the largest step of its tile would pass 2^14, and then to 2^6, so that the sums are seldom rescaled. The warps' parts are joined in shared memory, those of the
-// CTAs that share a long window by a second kernel, in a fixed order. A slot that is not seen has score -inf and its
-// step and lo are read as zeros, whatever it holds.
+//     with the largest step in view. They cross from the scores' layout to the operand's by movmatrix.
+// For float32 inputs queries and products are held in three bf16 terms and the codes as bf16 code - 7.5, around zero, and
+// the matrix unit's sums, which are cut off rather than rounded, are short: the output is within 1e-6 of its norm.
+// A reference r and the sum of the weights 2^(score - r) per warp and head in float32; r rises only when a weight
+// times the largest step of its tile would pass 2^14, and then to 2^6, so that the sums are seldom rescaled. The
+// warps' parts are joined in shared memory, those of the CTAs that share a long window by a second kernel, in a fixed
+// order. A slot that is not seen has score -inf and its step and lo are read as zeros, whatever it holds.
 #include <cmath>
 #include <type_traits>
 
@@ -45,10 +45,11 @@ struct Q4Attn {
   static constexpr int TILE = POS + TS * 8;
   static constexpr int AW = 8, STAGES = 2, CTAS = ctas_per_sm(DK);  // warps per CTA, tiles in flight per warp
   static constexpr int SMEM = AW * STAGES * TILE;
-  static constexpr int QT = sizeof(T) == 4 ? 2 : 1;  // f16 terms of a query
-  static constexpr int PT = sizeof(T) == 4 ? 3 : 1;              // terms of a weight's product: one f16, or three bf16
+  // float32 throughout: queries and the weights' products in three bf16 terms, codes as code - 7.5; else one f16 term
+  static constexpr bool EXACT = sizeof(T) == 4;
+  static constexpr int QT = EXACT ? 3 : 1, PT = QT;
   // the sum of lo times the queries' sums as one product in bf16: four groups, two terms
-  static constexpr bool LO_MMA = QT == 1 && (NG == 1 || NG == 2 || NG == 4);
+  static constexpr bool LO_MMA = !EXACT && (NG == 1 || NG == 2 || NG == 4);
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -93,12 +94,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float f16_value(float x) { return __half2float(__float2half_rn(x)); }
 
-// the low four bits of each half as a pair of bf16 numbers code - 8
+// the low four bits of each half as a pair of bf16 numbers code - 7.5: 16 + code by their place in the mantissa, less 23.5
 __device__ __forceinline__ uint32_t centred(uint32_t x) {
   uint32_t y;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"((x & 0x000f000fu) | 0x43004300u), "r"(0x43084308u));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(((x << 3) & 0x00780078u) | 0x41804180u), "r"(0x41bc41bcu));
   return y;
 }
 
@@ -337,10 +337,11 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
       for (int i = 0; i < GS / 4; ++i) top = fmaxf(top, fabsf(x[a][i]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // the power of two that brings the largest magnitude to [2^14, 2^15), and its inverse times 2^24
+    // the power of two that brings the largest magnitude to [2^14, 2^15), and its inverse over the products' unit
     const int e = top > 0.f ? (int)(__float_as_uint(top) >> 23) : 127;
     const float up = __uint_as_float((uint32_t)min(268 - e, 254) << 23);
-    const float down = ldexpf(1.0f, 24 - (min(268 - e, 254) - 127));
+    constexpr float UNIT = C::EXACT ? 1.f : 5.9604644775390625e-8f;  // what a product's code counts: 2^-24 in f16
+    const float down = ldexpf(1.0f, (C::EXACT ? 0 : 24) - (min(268 - e, 254) - 127));
 #pragma unroll
     for (int a = 0; a < NG; ++a) {
       sum[a] = 0.f;
@@ -355,13 +356,18 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
       constexpr int HALF = GS / 8;
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
-        float u[4] = {x[a][2 * s], x[a][2 * s + HALF], x[a][2 * s + 1] * 0.0625f, x[a][2 * s + 1 + HALF] * 0.0625f};
+        float u[4] = {x[a][2 * s], x[a][2 * s + HALF], x[a][2 * s + 1], x[a][2 * s + 1 + HALF]};
+        if constexpr (C::EXACT) {
 #pragma unroll
-        for (int r = 0; r < QT; ++r) {
-          qb[a][s][r][0] = pack_f16(u[0], u[1]);
-          qb[a][s][r][1] = pack_f16(u[2], u[3]);
+          for (int r = 0; r < QT; ++r) {
+            qb[a][s][r][0] = pack_bf16(u[0], u[1]);
+            qb[a][s][r][1] = pack_bf16(u[2], u[3]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) u[i] -= f16_value(u[i]);
+            for (int i = 0; i < 4; ++i) u[i] -= __bfloat162float(__float2bfloat16_rn(u[i]));
+          }
+        } else {
+          qb[a][s][0][0] = pack_f16(u[0], u[1]);
+          qb[a][s][0][1] = pack_f16(u[2] * 0.0625f, u[3] * 0.0625f);
         }
       }
     }
@@ -369,7 +375,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
       // k = 2 t holds a step (times zero), k = 2 t + 1 the lo of group t, times the group's query sum in two terms
       float mine_sum = 0.f;
 #pragma unroll
-      for (int a = 0; a < NG; ++a) mine_sum = t == a ? sum[a] * 5.9604644775390625e-8f : mine_sum;  // 2^-24
+      for (int a = 0; a < NG; ++a) mine_sum = t == a ? sum[a] * UNIT : mine_sum;
       const float hi = __bfloat162float(__float2bfloat16_rn(mine_sum));
       qlo[0] = pack_bf16(0.f, hi);
       qlo[1] = pack_bf16(0.f, mine_sum - hi);
@@ -380,7 +386,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
       const int from = 4 * (2 * t + c);
       f[c] = scale_log2 * __shfl_sync(0xffffffffu, down, from);
 #pragma unroll
-      for (int a = 0; a < NG; ++a) qs[a][c] = __shfl_sync(0xffffffffu, sum[a], from) * 5.9604644775390625e-8f;  // 2^-24
+      for (int a = 0; a < NG; ++a) qs[a][c] = __shfl_sync(0xffffffffu, sum[a], from) * UNIT;
     }
   }
 
@@ -483,10 +489,13 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
       } else {
 #pragma unroll
         for (int a = 0; a < NG; ++a) {
-          tot[0] = fmaf(q4_lo(p0[a]), qs[a][0], tot[0]);
-          tot[1] = fmaf(q4_lo(p0[a]), qs[a][1], tot[1]);
-          tot[2] = fmaf(q4_lo(p1[a]), qs[a][0], tot[2]);
-          tot[3] = fmaf(q4_lo(p1[a]), qs[a][1], tot[3]);
+          // with codes as code - 7.5, lo + 7.5 step takes the place of lo
+          const float lo0 = C::EXACT ? fmaf(7.5f, q4_step(p0[a]), q4_lo(p0[a])) : q4_lo(p0[a]);
+          const float lo1 = C::EXACT ? fmaf(7.5f, q4_step(p1[a]), q4_lo(p1[a])) : q4_lo(p1[a]);
+          tot[0] = fmaf(lo0, qs[a][0], tot[0]);
+          tot[1] = fmaf(lo0, qs[a][1], tot[1]);
+          tot[2] = fmaf(lo1, qs[a][0], tot[2]);
+          tot[3] = fmaf(lo1, qs[a][1], tot[3]);
         }
       }
 #pragma unroll
@@ -504,11 +513,17 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
 #pragma unroll
         for (int k = 0; k < KSTEPS; ++k) {
           const uint32_t x0 = w0 >> (8 * k), x1 = w1 >> (8 * k);
-          const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+          if constexpr (C::EXACT) {
+            const uint32_t a0 = centred(x0), a1 = centred(x1), a2 = centred(x0 >> 4), a3 = centred(x1 >> 4);
 #pragma unroll
-          for (int r = 0; r < QT; ++r) {
-            if (k == 0 && r == 0) mma_f16_first(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
-            else mma_f16(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+            for (int r = 0; r < QT; ++r) {
+              if (k == 0 && r == 0) mma_bf16_first(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+              else mma_bf16(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+            }
+          } else {
+            const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+            if (k == 0) mma_f16_first(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
+            else mma_f16(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
           }
         }
         const float s0 = q4_step(p0[a]), s1 = q4_step(p1[a]);
@@ -590,9 +605,9 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
 #pragma unroll
       for (int a = 0; a < NG; ++a) {
         const float st0 = q4_step(p0[a]), st1 = q4_step(p1[a]);
-        // with codes as code - 8, lo + 8 step takes the place of lo
-        const float lo0 = PT > 1 ? fmaf(8.f, st0, q4_lo(p0[a])) : q4_lo(p0[a]);
-        const float lo1 = PT > 1 ? fmaf(8.f, st1, q4_lo(p1[a])) : q4_lo(p1[a]);
+        // with codes as code - 7.5, lo + 7.5 step takes the place of lo
+        const float lo0 = PT > 1 ? fmaf(7.5f, st0, q4_lo(p0[a])) : q4_lo(p0[a]);
+        const float lo1 = PT > 1 ? fmaf(7.5f, st1, q4_lo(p1[a])) : q4_lo(p1[a]);
         low[a][0] = fmaf(s[mt][0], lo0, fmaf(s[mt][2], lo1, low[a][0]));
         low[a][1] = fmaf(s[mt][1], lo0, fmaf(s[mt][3], lo1, low[a][1]));
         float e[4] = {s[mt][0] * st0, s[mt][1] * st0, s[mt][2] * st1, s[mt][3] * st1};
@@ -617,8 +632,13 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
           const uint32_t y = __byte_perm(w[2][i16 / 4], w[3][i16 / 4], sel);
           if constexpr (PT > 1) {
             const uint32_t a0 = centred(x), a1 = centred(x >> 4), a2 = centred(y), a3 = centred(y >> 4);
+            // the matrix unit's sums are cut off, not rounded: a short one, then a rounded addition
+            float d[4];
+            mma_bf16_first(d, a0, a1, a2, a3, b0[0], b1[0]);
 #pragma unroll
-            for (int r = 0; r < PT; ++r) mma_bf16(acc[i16], a0, a1, a2, a3, b0[r], b1[r]);
+            for (int r = 1; r < PT; ++r) mma_bf16(d, a0, a1, a2, a3, b0[r], b1[r]);
+#pragma unroll
+            for (int e2 = 0; e2 < 4; ++e2) acc[i16][e2] += d[e2];
           } else {
             mma_f16(acc[i16], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, b0[0], b1[0]);
           }
