@@ -22,6 +22,7 @@ from torch import Tensor, nn
 
 from vesper_b200.contracts import ContractError, Dims, check_shape, require
 from vesper_b200.kernels.compact import Compaction, expand_rows, gather_rows
+from vesper_b200.kernels.q4_cache import Q4RingKVCache, q4_read, q4_ring_empty, q4_write_
 from vesper_b200.kernels.rotary import rotary
 from vesper_b200.kernels.window_attn import window_attention, window_attention_active
 
@@ -117,6 +118,33 @@ def ring_from_cache(cache: KVCache) -> RingKVCache:
         ring.pos.scatter_(1, slot, cache.pos)
         ring.valid.scatter_(1, slot, torch.ones_like(slot, dtype=torch.bool))
     return ring
+
+
+def cache_from_ring(ring: RingKVCache | Q4RingKVCache, last: Tensor, m: int, dtype: torch.dtype) -> KVCache:
+    """The chronological cache of the ``m`` positions up to ``last [b]`` (int64) that a ring holds: the switch from
+    one-token decoding back to chunks. ``m`` is at most the window and the number of tokens written."""
+    if not 0 <= m <= ring.window:
+        msg = f"m must lie in [0, {ring.window}], got {m}"
+        raise ValueError(msg)
+    pos = last[:, None] + torch.arange(1 - m, 1, device=last.device)
+    if isinstance(ring, Q4RingKVCache):
+        k, v, held = q4_read(ring, pos, dtype)
+    else:
+        b, _, hkv, dk = ring.k.shape
+        slot = pos % ring.window
+        at = slot[:, :, None, None].expand(b, m, hkv, dk)
+        k, v = ring.k.gather(1, at).to(dtype), ring.v.gather(1, at).to(dtype)
+        held = ring.valid.gather(1, slot) & (ring.pos.gather(1, slot) == pos)
+    if m:
+        require(held.all(), "cache_from_ring: the ring does not hold every position asked for")
+    return KVCache(k=k, v=v, pos=pos, window=ring.window)
+
+
+def q4_ring_from_cache(cache: KVCache) -> Q4RingKVCache:
+    """The 4-bit ring holding a chronological cache's entries (``ring_from_cache``, quantised)."""
+    b, _, hkv, dk = cache.k.shape
+    ring = q4_ring_empty(b, hkv, dk, cache.window, cache.k.device)
+    return q4_write_(ring, cache.k, cache.v, cache.pos)
 
 
 class WindowedAttention(nn.Module):

@@ -36,6 +36,7 @@ from vesper_b200.kernels.delta_scan import (
 )
 from vesper_b200.kernels.keys import fused_keys
 from vesper_b200.kernels.norm import add_rms_norm, fused_rms_norm
+from vesper_b200.kernels.q4_cache import Q4RingKVCache, q4_ring_empty
 from vesper_b200.kernels.rotary import inv_freq
 from vesper_b200.kernels.slabs import slab_ffn, slab_linears, slab_residual_norm
 
@@ -104,24 +105,30 @@ class ColumnState:
     ``key_history[t] [b,K-1,d]`` (``vesper/column.py:429-441``)."""
 
     h: tuple[Tensor, ...]
-    kv: tuple[KVCache | RingKVCache, ...]
+    kv: tuple[KVCache | RingKVCache | Q4RingKVCache, ...]
     key_history: tuple[Tensor, ...]
 
 
 def init_column_state(shape: ColumnShape, b: int, t_max: int, dtype: torch.dtype, device: torch.device, *,
-                      ring: bool = False) -> ColumnState:  # fmt: skip
+                      ring: bool = False, q4: bool = False) -> ColumnState:  # fmt: skip
     """Cold state (``vesper/column.py:444-480``): zero states and histories in
     ``promote_types(dtype, float32)``, empty windows in ``dtype`` (``ring``: unwritten rings for
-    one-token decoding)."""
+    one-token decoding, with ``q4`` rings held in 4 bits)."""
     if t_max < 1:
         msg = f"t_max must be at least 1, got {t_max}"
         raise ValueError(msg)
     dk = shape.head_dim
     sdt = torch.promote_types(dtype, torch.float32)
     empty = kv_ring_empty if ring else kv_cache_empty
+
+    def window() -> KVCache | RingKVCache | Q4RingKVCache:
+        if ring and q4:
+            return q4_ring_empty(b, shape.kv_heads, dk, shape.window, device)
+        return empty(b, shape.kv_heads, dk, shape.window, dtype, device)
+
     return ColumnState(
         h=tuple(torch.zeros(b, shape.heads, dk, dk, dtype=sdt, device=device) for _ in range(t_max)),
-        kv=tuple(empty(b, shape.kv_heads, dk, shape.window, dtype, device) for _ in range(t_max)),
+        kv=tuple(window() for _ in range(t_max)),
         key_history=tuple(torch.zeros(b, shape.key_history, shape.d, dtype=sdt, device=device) for _ in range(t_max)),
     )
 
@@ -129,7 +136,9 @@ def init_column_state(shape: ColumnShape, b: int, t_max: int, dtype: torch.dtype
 def map_state(state: ColumnState, f: Callable[[Tensor], Tensor]) -> ColumnState:
     """Every tensor of ``state`` through ``f`` in a fixed order (``vesper/column.py:500-517``)."""
 
-    def window(c: KVCache | RingKVCache) -> KVCache | RingKVCache:
+    def window(c: KVCache | RingKVCache | Q4RingKVCache) -> KVCache | RingKVCache | Q4RingKVCache:
+        if isinstance(c, Q4RingKVCache):
+            return Q4RingKVCache(f(c.k_codes), f(c.k_params), f(c.v_codes), f(c.v_params), f(c.pos), c.window)
         if isinstance(c, RingKVCache):
             return RingKVCache(k=f(c.k), v=f(c.v), pos=f(c.pos), valid=f(c.valid), window=c.window)
         return KVCache(k=f(c.k), v=f(c.v), pos=f(c.pos), window=c.window)

@@ -13,7 +13,11 @@ change and one captured graph serves every step.
 ``prefill`` is the long-context half: the prompt runs through the ordinary chunked forward
 (``Vesper.run`` with the dense rule, chronological ``KVCache`` windows, the chunked scan and
 window-attention kernels), chunk by chunk with carried states, and its windows are then moved into
-rings (``ring_from_cache``), so decoding continues exactly where the prompt ended.
+rings (``ring_from_cache``), so decoding continues exactly where the prompt ended. ``extend`` is the way
+back: the rings' windows become chronological caches again (``cache_from_ring``), more prompt runs
+through the chunked forward, and its tokens go into the rings.
+
+``quantized=True`` decodes with int8 products and rings held in 4 bits (``vesper_b200.quant``).
 """
 
 from __future__ import annotations
@@ -23,11 +27,13 @@ from collections.abc import Sequence
 import torch
 from torch import Tensor
 
-from vesper_b200.attention import ring_from_cache
+from vesper_b200.attention import KVCache, cache_from_ring, q4_ring_from_cache, ring_from_cache
 from vesper_b200.column import ColumnState, state_tensors
 from vesper_b200.contracts import ContractError
+from vesper_b200.kernels.q4_cache import Q4RingKVCache, q4_write_
 from vesper_b200.loop import DenseRule
 from vesper_b200.model import Vesper
+from vesper_b200.quant import QuantizedVesper
 
 
 def decode_forward(model: Vesper, token: Tensor, position: Tensor, states: Sequence[ColumnState], depth: int) -> Tensor:
@@ -60,15 +66,19 @@ class BatchedDecoder:
     ``prefill(tokens)`` runs a prompt ``[b, P]`` (positions ``0 .. P-1``) and returns the logits of
     every prompt position; ``step(token)`` advances every row by one token ``[b, 1]`` at the next
     position and returns ``(ids, logits)`` (the graph's buffers after a replay: read them before the
-    next step). ``dtype``: the activation dtype (bfloat16 runs under autocast with the chunked and
-    one-token bf16 kernels; float32 is the reference's precision).
+    next step). ``extend(tokens)`` runs more tokens of a prompt ``[b, P]`` at the positions that follow, after any
+    number of steps. ``dtype``: the activation dtype (bfloat16 runs under autocast with the chunked and
+    one-token bf16 kernels; float32 is the reference's precision). ``quantized``: the steps run int8
+    products over weights quantised here, once, and attend rings held in 4 bits; prompts run in ``dtype``
+    as ever, their windows quantised as they enter the rings.
 
     Raises:
-        ContractError: if the model is not on CUDA or ``depth`` is outside ``1..t_max``.
+        ContractError: if the model is not on CUDA or ``depth`` is outside ``1..t_max``, or ``quantized`` with a
+            head dimension that is not a multiple of 16 up to 128.
     """
 
     def __init__(self, model: Vesper, depth: int, vocab: int, b: int, dtype: torch.dtype = torch.bfloat16,
-                 warm: int = 2) -> None:  # fmt: skip
+                 warm: int = 2, *, quantized: bool = False) -> None:  # fmt: skip
         device = next(model.parameters()).device
         if device.type != "cuda":
             msg = f"the decoder runs on CUDA, the model is on {device}"
@@ -78,7 +88,9 @@ class BatchedDecoder:
             raise ContractError(msg)
         self.model, self.depth, self.vocab, self.b, self.dtype, self.warm = model, depth, vocab, b, dtype, warm
         self.device = device
-        self.states: list[ColumnState] = model.init_states(b, dtype, device, ring=True)
+        self.quant = QuantizedVesper(model, dtype) if quantized else None
+        self.states: list[ColumnState] = model.init_states(b, dtype, device, ring=True, q4=quantized)
+        self.length, self.last = 0, 0  # tokens so far, and the last one's position, of every row
         self.token = torch.zeros(b, 1, dtype=torch.long, device=device)
         self.position = torch.zeros(b, 1, dtype=torch.long, device=device)
         self.graph: torch.cuda.CUDAGraph | None = None
@@ -98,26 +110,85 @@ class BatchedDecoder:
         if b != self.b:
             msg = f"prompt of {b} rows for a decoder of {self.b}"
             raise ContractError(msg)
-        states = self.model.init_states(b, self.dtype, self.device)
-        outs = []
-        for s in range(0, length, chunk):
-            piece = tokens[:, s : s + chunk].to(self.device)
-            pos = torch.arange(s, s + piece.shape[1], device=self.device).expand(b, -1).contiguous()
-            with self._autocast():
-                res = self.model.run(piece, pos, states, passes=self.depth, exit_rule=DenseRule())
-                if all_logits or s + chunk >= length:
-                    outs.append(self.model.head(res.y if all_logits else res.y[:, -1:])[..., : self.vocab])
-            states = list(res.states)
-        rings = [ColumnState(h=s.h, kv=tuple(ring_from_cache(c) for c in s.kv), key_history=s.key_history)
+        logits, states = self._chunks(tokens, self.model.init_states(b, self.dtype, self.device), 0, chunk, all_logits)
+        to_ring = q4_ring_from_cache if self.quant else ring_from_cache
+        rings = [ColumnState(h=s.h, kv=tuple(to_ring(c) for c in s.kv), key_history=s.key_history)
                  for s in states]  # fmt: skip
         # into the decoder's own (possibly captured) buffers
         for dst, src in zip(state_tensors(self.states), state_tensors(rings), strict=True):
             dst.copy_(src)
         self.position.fill_(length - 1)
-        return torch.cat(outs, dim=1)
+        self.length, self.last = length, length - 1
+        return logits
+
+    def _chunks(self, tokens: Tensor, states: list[ColumnState], first: int, chunk: int,
+                all_logits: bool) -> tuple[Tensor, list[ColumnState]]:  # fmt: skip
+        """The chunked forward of ``tokens [b, P]`` from position ``first``: logits and new states."""
+        b, length = tokens.shape
+        outs = []
+        for s in range(0, length, chunk):
+            piece = tokens[:, s : s + chunk].to(self.device)
+            pos = torch.arange(first + s, first + s + piece.shape[1], device=self.device).expand(b, -1).contiguous()
+            with self._autocast():
+                res = self.model.run(piece, pos, states, passes=self.depth, exit_rule=DenseRule())
+                if all_logits or s + chunk >= length:
+                    outs.append(self.model.head(res.y if all_logits else res.y[:, -1:])[..., : self.vocab])
+            states = list(res.states)
+        return torch.cat(outs, dim=1), states
+
+    @torch.no_grad()
+    def extend(self, tokens: Tensor, chunk: int = 2048, *, all_logits: bool = False) -> Tensor:
+        """Run ``tokens [b, P]`` at the positions after every row's last one, as ``prefill`` runs a prompt.
+
+        The windows are read out of the rings (4-bit ones as the values they stand for), the chunked forward carries
+        them and the states on, and the new tokens are written into the rings; older entries of the rings stay as
+        they are. Returns logits as ``prefill`` does."""
+        b, length = tokens.shape
+        if b != self.b:
+            msg = f"prompt of {b} rows for a decoder of {self.b}"
+            raise ContractError(msg)
+        if self.length == 0:
+            return self.prefill(tokens, chunk, all_logits=all_logits)
+        if length == 0:
+            msg = "extend: at least one token is needed"
+            raise ContractError(msg)
+        last = self.position[:, 0]
+        caches = [
+            ColumnState(h=s.h, kv=tuple(cache_from_ring(c, last, min(self.length, c.window), self.dtype) for c in s.kv),
+                        key_history=s.key_history)
+            for s in self.states
+        ]  # fmt: skip
+        logits, states = self._chunks(tokens, caches, self.last + 1, chunk, all_logits)
+        for old, new in zip(self.states, states, strict=True):
+            for dst, src in zip((*old.h, *old.key_history), (*new.h, *new.key_history), strict=True):
+                dst.copy_(src)
+            for ring, cache in zip(old.kv, new.kv, strict=True):
+                self._into_ring(ring, cache, min(length, cache.window))
+        self.position.add_(length)
+        self.length, self.last = self.length + length, self.last + length
+        return logits
+
+    @staticmethod
+    def _into_ring(ring: object, cache: KVCache, n: int) -> None:
+        """The newest ``n`` entries of ``cache`` into ``ring``, in place."""
+        m = cache.k.shape[1]
+        k, v, pos = cache.k[:, m - n :], cache.v[:, m - n :], cache.pos[:, m - n :]
+        if isinstance(ring, Q4RingKVCache):
+            q4_write_(ring, k, v, pos)
+            return
+        slot = pos % ring.window
+        at = slot[:, :, None, None].expand_as(k)
+        ring.k.scatter_(1, at, k.to(ring.k.dtype))
+        ring.v.scatter_(1, at, v.to(ring.v.dtype))
+        ring.pos.scatter_(1, slot, pos)
+        ring.valid.scatter_(1, slot, torch.ones_like(slot, dtype=torch.bool))
 
     def _body(self) -> tuple[Tensor, Tensor]:
         self.position.add_(1)
+        if self.quant is not None:
+            x, r = self.quant.forward(self.token, self.position, self.states, self.depth)
+            logits = self.quant.logits(x, r)[..., : self.vocab]
+            return logits.argmax(-1), logits
         with self._autocast():
             return decode_step(self.model, self.depth, self.vocab, self.states, self.token, self.position)
 
@@ -141,6 +212,7 @@ class BatchedDecoder:
             self.graph.replay()
             out = self.outputs
         self.steps += 1
+        self.length, self.last = self.length + 1, self.last + 1
         return out
 
     def release(self) -> None:

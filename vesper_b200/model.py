@@ -54,8 +54,9 @@ class Vesper(nn.Module):
         self.norm_out = RMSNorm(shape.d)
         self.shape, self.columns, self.t_max = shape, columns, t_max
 
-    def init_states(self, b: int, dtype: torch.dtype, device: torch.device, *, ring: bool = False) -> list[ColumnState]:
-        return [init_column_state(self.shape, b, self.t_max, dtype, device, ring=ring) for _ in range(self.columns)]
+    def init_states(self, b: int, dtype: torch.dtype, device: torch.device, *, ring: bool = False,
+                    q4: bool = False) -> list[ColumnState]:  # fmt: skip
+        return [init_column_state(self.shape, b, self.t_max, dtype, device, ring=ring, q4=q4) for _ in range(self.columns)]
 
     def head(self, y: Tensor) -> Tensor:
         """Outputs ``[b, n, d]`` to logits ``[b, n, V]``: the output norm, then the tied embedding
