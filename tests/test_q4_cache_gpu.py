@@ -371,3 +371,43 @@ def test_refusals() -> None:
         q4_read(small, pos)
     with pytest.raises(ContractError, match="dtype: must be"):
         q4_read(ring, pos, torch.float64)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_offsets_past_32_bits(dtype: torch.dtype) -> None:
+    """A ring of 5 GB of key codes, its few tokens in the last head of the last row and across the ring's end."""
+    b, hkv, dk, window = 2, 8, 128, 5_000_000
+    ring = q4_ring_empty(b, hkv, dk, window, CUDA)
+    assert ring.k_codes.numel() > 2**32
+    n, last = 300, 2 * window + 100  # positions last - 299 .. last: slots window - 199 .. window - 1, 0 .. 100
+    k, v = _tokens(b, n, hkv, dk, 95, dtype)
+    pos = _positions([last - n + 1] * b, n)
+    q4_write_(ring, k.to(CUDA), v.to(CUDA), pos.to(CUDA))
+    k2, v2, held = q4_read(ring, pos.to(CUDA), torch.float32)
+    assert bool(held.all()) and torch.equal(k2.cpu(), _stored(k)[0]) and torch.equal(v2.cpu(), _stored(v)[0])
+    g = torch.Generator().manual_seed(96)
+    q = torch.randn(b, 1, 16, dk, generator=g).to(dtype).to(CUDA)
+    k1, v1 = (t.to(CUDA) for t in _tokens(b, 1, hkv, dk, 97, dtype))
+    at = torch.full((b, 1), last + 1, device=CUDA)
+    o = q4_attend_(q, k1, v1, at, ring)
+    all_k = torch.cat([_stored(k)[0], _stored(k1)[0]], 1).double()
+    all_v = torch.cat([_stored(v)[0], _stored(v1)[0]], 1).double()
+    qs = q[:, 0].double().cpu().view(b, hkv, 2, dk)
+    w = torch.softmax(torch.einsum("bhgd,blhd->bhgl", qs, all_k) / math.sqrt(dk), -1)
+    want = torch.einsum("bhgl,blhd->bhgd", w, all_v).reshape(b, 1, 16, dk)
+    for i in range(b):
+        assert rel(o[i].double().cpu().numpy(), want[i].numpy()) < TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows_of_uneven_lengths_share_the_work(dtype: torch.dtype) -> None:
+    """More rows than a warp has lanes, lengths from none to the window, and rows that attend nothing."""
+    b, hkv, window = 75, 2, 3000
+    held = [(i * 977) % 3100 for i in range(b)]
+    ring = _filled(b, hkv, 64, window, held, 98, dtype)
+    pos = [-1 if i % 11 == 5 else x for i, x in enumerate(held)]
+    _check_attend(ring, 4, pos, 99, dtype)
+    g = torch.Generator().manual_seed(3)
+    q, k = torch.randn(b, 1, 4, 64, generator=g).to(dtype).to(CUDA), torch.randn(b, 1, hkv, 64, generator=g).to(dtype).to(CUDA)
+    none = torch.full((b, 1), -1, device=CUDA)
+    assert not bool(q4_attend_(q, k, k, none, ring).any())  # nothing to share at all

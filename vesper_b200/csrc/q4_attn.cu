@@ -148,15 +148,19 @@ __device__ __forceinline__ int tiles_of(int64_t p, int W) {
   return p < 0 ? 0 : (int)((min(p + 1, (int64_t)W) + TS - 1) / TS);
 }
 
-// Where tile `at` of all rows' and units' tiles lies, in that order: its row, the row's first tile and number of
+// What a unit counts when the work is shared: its tiles, and `opening` more for what its opening and closing cost (the
+// queries, the first tiles' way from memory, the joining of the warps).
+__device__ __forceinline__ int cost_of(int tiles, int opening) { return tiles > 0 ? tiles + opening : 0; }
+
+// Where `at` lies among all rows' and units' costs, in that order: its row, where the row begins and its number of
 // tiles (per unit). Called by whole warps.
 template <int TS>
-__device__ __forceinline__ void find_row(const int64_t* pos, int B, int units, int W, int64_t at, int64_t& row,
-                                         int64_t& first, int& n) {
+__device__ __forceinline__ void find_row(const int64_t* pos, int B, int units, int W, int opening, int64_t at,
+                                         int64_t& row, int64_t& first, int& n) {
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
   for (int r0 = 0; r0 < B; r0 += 32) {
-    const int mine = r0 + lane < B ? tiles_of<TS>(pos[r0 + lane], W) : 0;
+    const int mine = r0 + lane < B ? cost_of(tiles_of<TS>(pos[r0 + lane], W), opening) : 0;
     int upto = mine;  // 32 rows of at most 2^25 tiles
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
@@ -167,8 +171,9 @@ __device__ __forceinline__ void find_row(const int64_t* pos, int B, int units, i
     if (past) {
       const int l = __ffs(past) - 1;
       row = r0 + l;
-      n = __shfl_sync(0xffffffffu, mine, l);
-      first = (before + __shfl_sync(0xffffffffu, upto, l) - n) * units;
+      const int cost = __shfl_sync(0xffffffffu, mine, l);
+      n = cost - opening;
+      first = (before + __shfl_sync(0xffffffffu, upto, l) - cost) * units;
       return;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
@@ -178,10 +183,11 @@ __device__ __forceinline__ void find_row(const int64_t* pos, int B, int units, i
   n = 0;
 }
 
-// All rows' and units' tiles, and how many of a launch's CTAs share them: as many as have a tile for each of their warps,
-// but one for each unit that sees something if that is more.
+// All rows' and units' costs, and how many of a launch's CTAs share them: as many as have a tile for each of their warps,
+// but one for each unit that sees something if that is more. An opening counts 16 tiles where a CTA has over 32 (8
+// streams of 6249 to 49999 positions, 8 key heads of 128: 61 us, with none 67, with 40 63), none where it has fewer.
 template <int TS, int AW>
-__device__ __forceinline__ int64_t all_tiles(const int64_t* pos, int B, int units, int W, int& ctas) {
+__device__ __forceinline__ int64_t all_costs(const int64_t* pos, int B, int units, int W, int& ctas, int& opening) {
   int64_t sum = 0;
   int live = 0;
   for (int r = threadIdx.x & 31; r < B; r += 32) {
@@ -192,12 +198,12 @@ __device__ __forceinline__ int64_t all_tiles(const int64_t* pos, int B, int unit
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
   live = __reduce_add_sync(0xffffffffu, live);
-  sum *= units;
-  ctas = (int)min((int64_t)ctas, max((sum + AW - 1) / AW, (int64_t)live * units));
-  return sum;
+  ctas = (int)min((int64_t)ctas, max((sum * units + AW - 1) / AW, (int64_t)live * units));
+  opening = sum * units > (int64_t)32 * ctas ? 16 : 0;
+  return (sum + (int64_t)live * opening) * units;
 }
 
-// `total` tiles in even parts: part i begins at floor(i total / parts)
+// `total` in even parts: part i begins at floor(i total / parts)
 struct Share {
   int64_t each;
   uint32_t rest, parts;
@@ -213,8 +219,8 @@ struct Share {
   __device__ __forceinline__ int64_t start(uint32_t i) const { return each * i + rest * i / parts; }
 };
 
-// A unit is eight query heads of one key head. With `shared` the CTAs divide all rows' and units' tiles evenly between
-// them, whatever the rows' lengths: CTA i takes tiles [i T / n, (i + 1) T / n) and writes what it has of a unit it does
+// A unit is eight query heads of one key head. With `shared` the CTAs divide all rows' and units' costs evenly between
+// them, whatever the rows' lengths: CTA i takes what lies in [i T / n, (i + 1) T / n) and writes what it has of a unit it does
 // not hold whole to its partials, [2 i] of the unit it starts within and [2 i + 1] of the one it ends within, each
 // [HEADS][DK + 2]: per head the unnormalised output, the reference and the sum; span[row][unit] gets the first and
 // the last CTA of a unit. Else a CTA per unit and row.
@@ -222,8 +228,8 @@ template <typename T, int DK>
 __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
     q4_attn_kernel(const T* __restrict__ q, int64_t q_row, int q_vec, const T* __restrict__ k_new, int64_t k_row,
                    const T* __restrict__ v_new, int64_t v_row, const int64_t* __restrict__ pos, Ring ring,
-                   T* __restrict__ o, float* __restrict__ part, int2* __restrict__ span, int shared, int B, int H, int HKV, int head_tiles, int W,
-                   int SLOTS, float scale_log2) {
+                   T* __restrict__ o, float* __restrict__ part, int2* __restrict__ span, int shared, int B, int H,
+                   int HKV, int head_tiles, int W, int SLOTS, float scale_log2) {
   using C = Q4Attn<T, DK>;
   constexpr int GS = C::GS, NG = C::NG, QT = C::QT, PT = C::PT, TILES = DK / 16, KSTEPS = GS / 16, AW = C::AW;
   constexpr int TS = C::TS, MT = C::MT;
@@ -233,26 +239,29 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
   uint8_t* mine = smem + warp * C::STAGES * C::TILE;
   grid_wait();
   grid_release();
-  int64_t b = blockIdx.y, from = 0, until = 1, row_first = 0;  // tiles [from, until) of all, the row's first
-  int n = 0, unit = blockIdx.x, lo_t = 0, hi_t = 0;  // tiles of a unit of row b, and those of them this CTA has
+  int64_t b = blockIdx.y, from = 0, until = 1, row_first = 0;  // this CTA's share, and where row b begins
+  int opening = 0, n = 0, unit = blockIdx.x, lo_t = 0, hi_t = 0;  // tiles of a unit of row b, and those of them this CTA has
   if (shared) {
     int ctas = gridDim.x;
-    const int64_t total = all_tiles<TS, AW>(pos, B, units, W, ctas);
+    const int64_t total = all_costs<TS, AW>(pos, B, units, W, ctas, opening);
     if (blockIdx.x >= ctas) return;
     const Share share(total, ctas);
     from = share.start(blockIdx.x);
     until = share.start(blockIdx.x + 1);
-    find_row<TS>(pos, B, units, W, from, b, row_first, n);
+    find_row<TS>(pos, B, units, W, opening, from, b, row_first, n);
   }
   while (from < until) {
   int64_t p = 0;
   if (shared) {
     p = pos[b];
-    unit = from - row_first < ((int64_t)1 << 32) ? (int)((uint32_t)(from - row_first) / (uint32_t)n)
-                                                 : (int)((from - row_first) / n);
-    lo_t = (int)(from - row_first - (int64_t)unit * n);
-    hi_t = (int)min((int64_t)n, lo_t + (until - from));
-    from += hi_t - lo_t;
+    const int cost = cost_of(n, opening);
+    unit = from - row_first < ((int64_t)1 << 32) ? (int)((uint32_t)(from - row_first) / (uint32_t)cost)
+                                                 : (int)((from - row_first) / cost);
+    const int lo = (int)(from - row_first - (int64_t)unit * cost), hi = (int)min((int64_t)cost, lo + (until - from));
+    from += hi - lo;
+    lo_t = max(0, lo - opening);
+    hi_t = max(0, hi - opening);
+    if (lo_t >= hi_t) break;  // the share ends within a unit's opening
   } else {
     hi_t = SLOTS / TS;  // until the position has come: the first copies do not wait for it
     from = until;
@@ -708,7 +717,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
   // the next unit: its copies come into what was just read
   __syncthreads();
   if (hi_t == n && unit + 1 == units) {  // the next row that sees something
-    row_first += (int64_t)n * units;
+    row_first += (int64_t)cost_of(n, opening) * units;
     do n = tiles_of<TS>(pos[++b], W);
     while (n == 0);
   }

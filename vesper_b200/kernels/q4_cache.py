@@ -34,6 +34,7 @@ from vesper_b200.kernels.q8 import serving_only
 SUPPORTED = (torch.float32, torch.bfloat16, torch.float16)
 MAX_HEAD_DIM = 128
 SLOT_TILE = 64  # slots are allocated in whole tiles
+MAX_SLOTS = 2**31 - SLOT_TILE
 
 
 def group_size(dk: int) -> int:
@@ -63,8 +64,8 @@ class Q4RingKVCache:
 
 def q4_ring_empty(b: int, hkv: int, dk: int, window: int, device: torch.device) -> Q4RingKVCache:
     """Every slot unwritten (position -1)."""
-    if window < 1:
-        msg = f"window must be at least 1, got {window}"
+    if not 1 <= window <= MAX_SLOTS:
+        msg = f"window must be at least 1 and at most {MAX_SLOTS}, got {window}"
         raise ValueError(msg)
     if dk % 16 != 0 or not 16 <= dk <= MAX_HEAD_DIM:
         msg = f"head dimension {dk} must be a multiple of 16 and not exceed {MAX_HEAD_DIM}"
@@ -91,7 +92,7 @@ def _check_ring(ring: Q4RingKVCache, what: str) -> tuple[int, int, int, int]:
         b, hkv, slots, half = shape
         params = (b, hkv, slots, half // 16 if half % 16 == 0 else half // 8, 2)
         if (
-            half % 8 == 0 and 8 <= half <= MAX_HEAD_DIM // 2 and slots % SLOT_TILE == 0 and slots >= ring.window >= 1
+            half % 8 == 0 and 8 <= half <= MAX_HEAD_DIM // 2 and slots % SLOT_TILE == 0 and MAX_SLOTS >= slots >= ring.window >= 1
             and vc.shape == shape and kp.shape == params and vp.shape == params and pos.shape == (b, slots)
             and kc.dtype == torch.uint8 == vc.dtype and kp.dtype == torch.bfloat16 == vp.dtype and pos.dtype == torch.int64
             and kc.is_cuda and kp.device == device and vc.device == device and vp.device == device and pos.device == device
@@ -110,8 +111,8 @@ def _explain_ring(ring: Q4RingKVCache, what: str) -> tuple[int, int, int, int]:
     if dk % 16 != 0 or not 16 <= dk <= MAX_HEAD_DIM:
         msg = f"head dimension {dk} must be a multiple of 16 and not exceed {MAX_HEAD_DIM}"
         raise ContractError(msg)
-    if ring.window < 1 or slots % SLOT_TILE or slots < ring.window:
-        msg = f"ring: {slots} slots must be a multiple of {SLOT_TILE} holding the window {ring.window}"
+    if ring.window < 1 or slots % SLOT_TILE or slots < ring.window or slots > MAX_SLOTS:
+        msg = f"ring: {slots} slots must be a multiple of {SLOT_TILE} up to {MAX_SLOTS} holding the window {ring.window}"
         raise ContractError(msg)
     params = ("b", "hkv", "slots", dk // group_size(dk), 2)
     check_shape("ring.k_params", ring.k_params, params, dims, torch.bfloat16)

@@ -30,6 +30,7 @@ from vesper_b200.contracts import ContractError, Dims, check_shape, require_cuda
 
 SUPPORTED = (torch.float32, torch.bfloat16, torch.float16)
 MAX_K = 131056  # largest inner dimension whose int8 sums stay in int32
+MAX_ROWS = 2**31 - 1  # rows of either operand
 
 
 def serving_only(what: str, *tensors: Tensor) -> None:
@@ -201,7 +202,8 @@ def dequantize_rows_q8(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.floa
         pitch = flat.stride(0) if rows > 1 else width
     y = torch.empty(q.shape, dtype=dtype, device=q.device)
     _lib.call(
-        "vb_dequantize_rows_q8", flat.data_ptr(), pitch, scale.contiguous().data_ptr(), y.data_ptr(), rows, width, _lib.DTYPE_CODE[dtype], _lib.stream(q.device),
+        "vb_dequantize_rows_q8", flat.data_ptr(), pitch, scale.contiguous().data_ptr(), y.data_ptr(), rows, width,
+        _lib.DTYPE_CODE[dtype], _lib.stream(q.device),
     )  # fmt: skip
     return y
 
@@ -211,7 +213,7 @@ def _check_linear(xq: Tensor, xs: Tensor, wq: Tensor, ws: Tensor, out_dtype: tor
     device = xq.device
     if (
         wq.dim() == 2 and xq.dim() >= 1 and wq.dtype == torch.int8 == xq.dtype and xs.dtype == torch.float32 == ws.dtype
-        and 1 <= wq.shape[1] <= MAX_K and xq.shape[-1] == wq.shape[1] and xs.shape == xq.shape[:-1]
+        and 1 <= wq.shape[1] <= MAX_K and wq.shape[0] <= MAX_ROWS and xs.numel() <= MAX_ROWS and xq.shape[-1] == wq.shape[1] and xs.shape == xq.shape[:-1]
         and ws.shape == wq.shape[:1] and wq.shape[0] >= 1 and out_dtype in SUPPORTED and xq.is_cuda
         and xs.device == device and wq.device == device and ws.device == device
     ):  # fmt: skip
@@ -229,7 +231,8 @@ def _check_linear(xq: Tensor, xs: Tensor, wq: Tensor, ws: Tensor, out_dtype: tor
         msg = f"out_dtype: must be one of {SUPPORTED}, got {out_dtype}"
         raise ContractError(msg)
     require_cuda("int8 product", xq, xs=xs, wq=wq, ws=ws)
-    msg = f"wq: expected at least one row of 1 to {MAX_K} channels, got shape {tuple(wq.shape)}"
+    msg = (f"wq: expected 1 to {MAX_ROWS} rows of 1 to {MAX_K} channels for at most {MAX_ROWS} rows of xq, got shape "
+           f"{tuple(wq.shape)} for {tuple(xq.shape)}")  # fmt: skip
     raise ContractError(msg)
 
 
