@@ -98,22 +98,22 @@ __device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t w) {
 }
 
 // The codes of eight channels, the first in the low four bits: rint of the correctly rounded quotient
-// (x - lo) / step, which is at most 15 (step is not below span / 15). Adding 1.5 * 2^23 rounds to whole
-// numbers; sums of four codes times powers of 16 are exact in float32. Step 0 or NaN gives zeros.
+// (x - lo) / step, which is at most 15 (step is not below span / 15). Adding 1.5 * 2^23 rounds to whole numbers, which
+// then lie in the lowest bits of the float. Step 0 or NaN gives zeros.
 __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float step, float lo, float inverse) {
   const uint64_t minus_lo = pair_f32(-lo, -lo), minus_step = pair_f32(-step, -step), r = pair_f32(inverse, inverse);
-  const uint64_t whole = pair_f32(12582912.0f, 12582912.0f), back = pair_f32(-12582912.0f, -12582912.0f);
-  uint64_t c[4];  // codes e and e + 4
+  const uint64_t whole = pair_f32(12582912.0f, 12582912.0f);
+  uint32_t w0 = 0, w1 = 0;  // codes 0 to 3 and 4 to 7, in the low halves
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 3; e >= 0; --e) {
     const uint64_t t = add2(pair_f32(x[e], x[e + 4]), minus_lo);
     const uint64_t q = mul2(t, r);
-    c[e] = add2(add2(fma2(fma2(q, minus_step, t), r, q), whole), back);
+    const uint64_t c = add2(fma2(fma2(q, minus_step, t), r, q), whole);
+    uint32_t c0, c1;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(c0), "=r"(c1) : "l"(c));
+    w0 = w0 * 16 + c0;
+    w1 = w1 * 16 + c1;
   }
-  const uint64_t sixteen = pair_f32(16.f, 16.f), bits = pair_f32(256.f, 256.f);
-  const uint64_t sum = add2(fma2(fma2(c[3], sixteen, c[2]), bits, fma2(c[1], sixteen, c[0])), pair_f32(8388608.f, 8388608.f));
-  uint32_t w0, w1;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(w0), "=r"(w1) : "l"(sum));
   return step > 0.f ? __byte_perm(w0, w1, 0x5410) : 0u;
 }
 

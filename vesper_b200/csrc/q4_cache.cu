@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(NT) q4_write_kernel(Q4Ring ring, const T* __re
   __shared__ int slots[ROWS];  // -1: not written
   // consecutive CTAs take consecutive tokens of a head, whose slots they fill side by side (4 x 32701 tokens, 8 heads of
   // 128: 170 us; with a token's heads next to each other 186)
-  const int tid = threadIdx.x, blocks = gridDim.x / HKV, kh = blockIdx.x / blocks, block = blockIdx.x - kh * blocks;
-  const int64_t b = blockIdx.y;
+  const int tid = threadIdx.x, block = blockIdx.x, kh = blockIdx.y;
+  const int64_t b = blockIdx.z;
   const int row0 = tid / PER, c0 = tid % PER * 8;
   const bool busy = RP * PER == NT || tid < RP * PER;
   grid_wait();
@@ -259,7 +259,7 @@ int check_ring(const char* what, int B, int N, int HKV, int DK, int W, int SLOTS
   VB_REQUIRE(SLOTS % Q4_TILE == 0 && SLOTS >= W, "%s: %d slots must be a multiple of %d holding the window %d", what,
              SLOTS, Q4_TILE, W);
   VB_REQUIRE(dtype_size(dtype) > 0, "%s: unsupported dtype code %d", what, dtype);
-  VB_REQUIRE(B <= 65535 && (int64_t)N * HKV < (int64_t(1) << 31), "%s: %d rows of %d tokens x %d key heads exceed the grid",
+  VB_REQUIRE(B <= 65535 && HKV <= 65535 && (int64_t)N * HKV < (int64_t(1) << 31), "%s: %d rows of %d tokens x %d key heads exceed the grid",
              what, B, N, HKV);
   return VB_OK;
 }
@@ -300,7 +300,7 @@ extern "C" int vb_q4_write(void* k_codes, void* k_params, void* v_codes, void* v
                   v_batch * size % 16 == 0 && v_token * size % 16 == 0;
   return VB_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return with_head_dim(DK, [&](auto dk) -> int {
-      return launch_early("q4_write", q4_write_kernel<T, decltype(dk)::value>, dim3((min(N, W) + Layout<decltype(dk)::value>::ROWS - 1) / Layout<decltype(dk)::value>::ROWS * HKV, B), NT,
+      return launch_early("q4_write", q4_write_kernel<T, decltype(dk)::value>, dim3((min(N, W) + Layout<decltype(dk)::value>::ROWS - 1) / Layout<decltype(dk)::value>::ROWS, HKV, B), NT,
                           0, 1, (cudaStream_t)stream, ring, (const T*)k, k_batch, k_token, (const T*)v, v_batch, v_token, pos,
                           vec, N, HKV, W, SLOTS);
     });
