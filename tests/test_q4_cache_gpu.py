@@ -288,6 +288,21 @@ def test_sharp_and_large_scores(dtype: torch.dtype) -> None:
     _check_attend(zero, 4, [99, 99], 77, dtype, scale=0.0)
 
 
+@pytest.mark.parametrize("size", [2.0**-20, 1.0, 2.0**40])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tiles_of_constant_values_among_large_ones(dtype: torch.dtype, size: float) -> None:
+    """Whole tiles of zeros (no step at all) before, between and after others: they take their weight's part."""
+    b, hkv, dk, window = 2, 1, 64, 1200
+    k, v = _tokens(b, window, hkv, dk, 78, dtype)
+    v = v * size
+    v[:, :70] = 0
+    v[:, 500:800] = 0
+    v[:, 1100:] = 0
+    pos = _positions([0, 0], window).to(CUDA)
+    ring = q4_write_(q4_ring_empty(b, hkv, dk, window, CUDA), k.to(CUDA), v.to(CUDA), pos)
+    _check_attend(ring, 4, [window - 1, window + 5], 79, dtype)
+
+
 def test_strided_tokens_and_streams() -> None:
     b, h, hkv, dk = 4, 8, 2, 64
     ring1, ring2 = (_filled(b, hkv, dk, 96, [95, 96, 97, 10], 80, torch.bfloat16) for _ in range(2))
@@ -323,6 +338,13 @@ def test_steps_in_a_graph() -> None:
         assert torch.equal(out, q4_attend_(q, k, v, pos, eager))
         pos.add_(1)
     assert torch.equal(ring.pos, eager.pos)
+
+
+def test_a_ring_without_key_heads_is_refused() -> None:
+    ring = q4_ring_empty(2, 0, 64, 64, CUDA)
+    q, kv = torch.zeros(2, 1, 4, 64, device=CUDA), torch.zeros(2, 1, 0, 64, device=CUDA)
+    with pytest.raises(ContractError, match="key heads"):
+        q4_attend_(q, kv, kv, torch.zeros(2, 1, dtype=torch.long, device=CUDA), ring)
 
 
 def test_empty_batches_and_chunks() -> None:

@@ -21,6 +21,14 @@
 // times the largest step of its tile would pass 2^14, and then to 2^6, so that the sums are seldom rescaled. The
 // warps' parts are joined in shared memory, those of the CTAs that share a long window by a second kernel, in a fixed
 // order. A slot that is not seen has score -inf and its step and lo are read as zeros, whatever it holds.
+//
+// Measured (bf16, device): 8 rows of 6249 to 49999 positions, 32 query and 8 key heads of 128, 61.5 us (290 MB, 4.7
+// TB/s, 72 % of a plain copy's rate); 8 x 32768 69.7 us (4.85 TB/s, 74 %). What keeps it from the copy's rate is
+// latency: eight warps an SM (238 registers each at DK 128) issue in half of the cycles, and the last tiles of a unit, the
+// joining of its warps and the next unit's first tiles follow one another. At DK 64, eight query heads to two key heads,
+// 64 x 8192 take 30.3 us (88 MB, 44 %): half the bytes for each instruction. 64 rows of 512 positions take 5.2 us, the
+// latency of position, tiles, two products and the joining. One float32 row of 100003 positions at DK 64, its
+// products nine times over, takes 21 us.
 #include <cmath>
 #include <type_traits>
 
@@ -251,476 +259,477 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
     find_row<TS>(pos, B, units, W, opening, from, b, row_first, n);
   }
   while (from < until) {
-  int64_t p = 0;
-  if (shared) {
-    p = pos[b];
-    const int cost = cost_of(n, opening);
-    unit = from - row_first < ((int64_t)1 << 32) ? (int)((uint32_t)(from - row_first) / (uint32_t)cost)
-                                                 : (int)((from - row_first) / cost);
-    const int lo = (int)(from - row_first - (int64_t)unit * cost), hi = (int)min((int64_t)cost, lo + (until - from));
-    from += hi - lo;
-    lo_t = max(0, lo - opening);
-    hi_t = max(0, hi - opening);
-    if (lo_t >= hi_t) break;  // the share ends within a unit's opening
-  } else {
-    hi_t = SLOTS / TS;  // until the position has come: the first copies do not wait for it
-    from = until;
-  }
-  const int kh = unit / head_tiles, ht = unit - kh * head_tiles, h0 = kh * G + ht * HEADS, heads = min(HEADS, G - ht * HEADS);
-  const int64_t base = (b * HKV + kh) * SLOTS;
-  // queries: thread (g, t) holds head g's channels of every group that the key codes of lane part t belong to. They and
-  // the token are loaded before the cache's tiles, behind which they would wait
-  __align__(16) T xraw[NG * (GS / 4)], tokraw[8];  // as they come: nothing waits for them before the copies are issued
-  {
-    const T* src = q + b * q_row + (int64_t)(h0 + min(g, heads - 1)) * DK + t * (GS / 4);
-    constexpr int BYTES = GS / 4 * (int)sizeof(T);
-    if (q_vec) {  // rows on 16-byte boundaries
-#pragma unroll
-      for (int a = 0; a < NG; ++a) {
-        if constexpr (BYTES == 8) reinterpret_cast<uint2*>(xraw)[a] = __ldg(reinterpret_cast<const uint2*>(src + a * GS));
-        else
-#pragma unroll
-          for (int i = 0; i < BYTES / 16; ++i)
-            reinterpret_cast<uint4*>(xraw)[a * (BYTES / 16) + i] = __ldg(reinterpret_cast<const uint4*>(src + a * GS) + i);
-      }
+    int64_t p = 0;
+    if (shared) {
+      p = pos[b];
+      const int cost = cost_of(n, opening);
+      unit = from - row_first < ((int64_t)1 << 32) ? (int)((uint32_t)(from - row_first) / (uint32_t)cost)
+                                                   : (int)((from - row_first) / cost);
+      const int lo = (int)(from - row_first - (int64_t)unit * cost), hi = (int)min((int64_t)cost, lo + (until - from));
+      from += hi - lo;
+      lo_t = max(0, lo - opening);
+      hi_t = max(0, hi - opening);
+      if (lo_t >= hi_t) break;  // the share ends within a unit's opening
     } else {
+      hi_t = SLOTS / TS;  // until the position has come: the first copies do not wait for it
+      from = until;
+    }
+    const int kh = unit / head_tiles, ht = unit - kh * head_tiles, h0 = kh * G + ht * HEADS, heads = min(HEADS, G - ht * HEADS);
+    const int64_t base = (b * HKV + kh) * SLOTS;
+    // queries: thread (g, t) holds head g's channels of every group that the key codes of lane part t belong to. They and
+    // the token are loaded before the cache's tiles, behind which they would wait
+    __align__(16) T xraw[NG * (GS / 4)], tokraw[8];  // as they come: nothing waits for them before the copies are issued
+    {
+      const T* src = q + b * q_row + (int64_t)(h0 + min(g, heads - 1)) * DK + t * (GS / 4);
+      constexpr int BYTES = GS / 4 * (int)sizeof(T);
+      if (q_vec) {  // rows on 16-byte boundaries
+#pragma unroll
+        for (int a = 0; a < NG; ++a) {
+          if constexpr (BYTES == 8) reinterpret_cast<uint2*>(xraw)[a] = __ldg(reinterpret_cast<const uint2*>(src + a * GS));
+          else
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i)
+              reinterpret_cast<uint4*>(xraw)[a * (BYTES / 16) + i] = __ldg(reinterpret_cast<const uint4*>(src + a * GS) + i);
+        }
+      } else {
+#pragma unroll
+        for (int a = 0; a < NG; ++a)
+#pragma unroll
+          for (int i = 0; i < GS / 4; ++i) xraw[a * (GS / 4) + i] = src[a * GS + i];
+      }
+    }
+    // the token: lane c < 16 holds eight channels of the key, 16 + c of the value
+    const bool tok_value = lane >= 16;
+    const int tok_c = (lane & 15) * 8;
+    if (tok_c < DK) {
+      const T* src = tok_value ? v_new + b * v_row + (int64_t)kh * DK + tok_c : k_new + b * k_row + (int64_t)kh * DK + tok_c;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) tokraw[i] = src[i];
+    }
+    auto copy = [&](int i) {  // tile lo_t + warp + 8 i into stage i mod 2; the group is committed even if it is empty
+      const int tile = lo_t + warp + AW * i;
+      if (tile < hi_t) {
+        const uint32_t to = smem_u32(mine + (i % C::STAGES) * C::TILE) + 16 * lane;
+        const int64_t s0 = base + (int64_t)tile * TS;
+        const uint8_t* kc = ring.k_codes + s0 * C::CODES + 16 * lane;
+        const uint8_t* vc = ring.v_codes + s0 * C::CODES + 16 * lane;
+        const uint8_t* kp = reinterpret_cast<const uint8_t*>(ring.k_params + s0 * NG) + 16 * lane;
+        const uint8_t* vp = reinterpret_cast<const uint8_t*>(ring.v_params + s0 * NG) + 16 * lane;
+#pragma unroll
+        for (int x = 0; x < C::VC; x += 512) cp_async16(to + x, kc + x, 16);
+#pragma unroll
+        for (int x = 0; x < TS * C::PAR; x += 512)
+          if (x + 512 <= TS * C::PAR || x + 16 * lane < TS * C::PAR) {
+            cp_async16(to + C::KP + x, kp + x, 16);
+            cp_async16(to + C::VP + x, vp + x, 16);
+          }
+        cp_async16(to + C::POS, reinterpret_cast<const uint8_t*>(ring.pos + b * SLOTS + (int64_t)tile * TS) + 16 * lane, 16);
+#pragma unroll
+        for (int x = 0; x < C::VC; x += 512) cp_async16(to + C::VC + x, vc + x, 16);
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < C::STAGES; ++i) copy(i);
+
+    if (!shared) {
+      p = pos[b];
+      n = hi_t = tiles_of<TS>(p, W);
+    }
+    const int own = p < 0 ? -1 : p < ((int64_t)1 << 31) ? (int)((uint32_t)p % (uint32_t)W) : (int)(p % W);
+    const int own_at = own >= 0 ? own / TS - lo_t : -1;  // the warp whose tile holds the token's slot has it
+    const bool has_own = own_at >= 0 && own / TS < hi_t && own_at % AW == warp;
+
+    uint32_t qb[NG][KSTEPS][QT][2], qlo[2] = {0u, 0u};
+    float qs[NG][2], f[2];
+    {
+      float x[NG][GS / 4], top = 0.f, sum[NG];
 #pragma unroll
       for (int a = 0; a < NG; ++a)
 #pragma unroll
-        for (int i = 0; i < GS / 4; ++i) xraw[a * (GS / 4) + i] = src[a * GS + i];
-    }
-  }
-  // the token: lane c < 16 holds eight channels of the key, 16 + c of the value
-  const bool tok_value = lane >= 16;
-  const int tok_c = (lane & 15) * 8;
-  if (tok_c < DK) {
-    const T* src = tok_value ? v_new + b * v_row + (int64_t)kh * DK + tok_c : k_new + b * k_row + (int64_t)kh * DK + tok_c;
+        for (int i = 0; i < GS / 4; ++i) x[a][i] = g < heads ? to_f32<T>(xraw[a * (GS / 4) + i]) : 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) tokraw[i] = src[i];
-  }
-  auto copy = [&](int i) {  // tile lo_t + warp + 8 i into stage i mod 2; the group is committed even if it is empty
-    const int tile = lo_t + warp + AW * i;
-    if (tile < hi_t) {
-      const uint32_t to = smem_u32(mine + (i % C::STAGES) * C::TILE) + 16 * lane;
-      const int64_t s0 = base + (int64_t)tile * TS;
-      const uint8_t* kc = ring.k_codes + s0 * C::CODES + 16 * lane;
-      const uint8_t* vc = ring.v_codes + s0 * C::CODES + 16 * lane;
-      const uint8_t* kp = reinterpret_cast<const uint8_t*>(ring.k_params + s0 * NG) + 16 * lane;
-      const uint8_t* vp = reinterpret_cast<const uint8_t*>(ring.v_params + s0 * NG) + 16 * lane;
+      for (int a = 0; a < NG; ++a)
 #pragma unroll
-      for (int x = 0; x < C::VC; x += 512) cp_async16(to + x, kc + x, 16);
-#pragma unroll
-      for (int x = 0; x < TS * C::PAR; x += 512)
-        if (x + 512 <= TS * C::PAR || x + 16 * lane < TS * C::PAR) {
-          cp_async16(to + C::KP + x, kp + x, 16);
-          cp_async16(to + C::VP + x, vp + x, 16);
-        }
-      cp_async16(to + C::POS, reinterpret_cast<const uint8_t*>(ring.pos + b * SLOTS + (int64_t)tile * TS) + 16 * lane, 16);
-#pragma unroll
-      for (int x = 0; x < C::VC; x += 512) cp_async16(to + C::VC + x, vc + x, 16);
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < C::STAGES; ++i) copy(i);
-
-  if (!shared) {
-    p = pos[b];
-    n = hi_t = tiles_of<TS>(p, W);
-  }
-  const int own = p < 0 ? -1 : p < ((int64_t)1 << 31) ? (int)((uint32_t)p % (uint32_t)W) : (int)(p % W);
-  const int own_at = own >= 0 ? own / TS - lo_t : -1;  // the warp whose tile holds the token's slot has it
-  const bool has_own = own_at >= 0 && own / TS < hi_t && own_at % AW == warp;
-
-  uint32_t qb[NG][KSTEPS][QT][2], qlo[2] = {0u, 0u};
-  float qs[NG][2], f[2];
-  {
-    float x[NG][GS / 4], top = 0.f, sum[NG];
-#pragma unroll
-    for (int a = 0; a < NG; ++a)
-#pragma unroll
-      for (int i = 0; i < GS / 4; ++i) x[a][i] = g < heads ? to_f32<T>(xraw[a * (GS / 4) + i]) : 0.f;
-#pragma unroll
-    for (int a = 0; a < NG; ++a)
-#pragma unroll
-      for (int i = 0; i < GS / 4; ++i) top = fmaxf(top, fabsf(x[a][i]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // the power of two that brings the largest magnitude to [2^14, 2^15), and its inverse over the products' unit
-    const int e = top > 0.f ? (int)(__float_as_uint(top) >> 23) : 127;
-    const float up = __uint_as_float((uint32_t)min(268 - e, 254) << 23);
-    constexpr float UNIT = C::EXACT ? 1.f : 5.9604644775390625e-8f;  // what a product's code counts: 2^-24 in f16
-    const float down = ldexpf(1.0f, (C::EXACT ? 0 : 24) - (min(268 - e, 254) - 127));
-#pragma unroll
-    for (int a = 0; a < NG; ++a) {
-      sum[a] = 0.f;
-#pragma unroll
-      for (int i = 0; i < GS / 4; ++i) {
-        x[a][i] *= up;
-        sum[a] += x[a][i];
-      }
-      sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 1);
-      sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 2);
-      // nibbles (i, i + half) share a register: halves of a word of eight codes, or of four for groups of 16
-      constexpr int HALF = GS / 8;
-#pragma unroll
-      for (int s = 0; s < KSTEPS; ++s) {
-        float u[4] = {x[a][2 * s], x[a][2 * s + HALF], x[a][2 * s + 1], x[a][2 * s + 1 + HALF]};
-        if constexpr (C::EXACT) {
-#pragma unroll
-          for (int r = 0; r < QT; ++r) {
-            qb[a][s][r][0] = pack_bf16(u[0], u[1]);
-            qb[a][s][r][1] = pack_bf16(u[2], u[3]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] -= __bfloat162float(__float2bfloat16_rn(u[i]));
-          }
-        } else {
-          qb[a][s][0][0] = pack_f16(u[0], u[1]);
-          qb[a][s][0][1] = pack_f16(u[2] * 0.0625f, u[3] * 0.0625f);
-        }
-      }
-    }
-    if constexpr (C::LO_MMA) {
-      // k = 2 t holds a step (times zero), k = 2 t + 1 the lo of group t, times the group's query sum in two terms
-      float mine_sum = 0.f;
-#pragma unroll
-      for (int a = 0; a < NG; ++a) mine_sum = t == a ? sum[a] * UNIT : mine_sum;
-      const float hi = __bfloat162float(__float2bfloat16_rn(mine_sum));
-      qlo[0] = pack_bf16(0.f, hi);
-      qlo[1] = pack_bf16(0.f, mine_sum - hi);
-    }
-    // what the sums' layout needs: heads 2 t and 2 t + 1
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int from = 4 * (2 * t + c);
-      f[c] = scale_log2 * __shfl_sync(0xffffffffu, down, from);
-#pragma unroll
-      for (int a = 0; a < NG; ++a) qs[a][c] = __shfl_sync(0xffffffffu, sum[a], from) * UNIT;
-    }
-  }
-
-  uint32_t tok_codes = 0, tok_params = 0;
-  if (has_own) {  // quantised, and written to the ring once per key head
-    float tok[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) tok[j] = tok_c < DK ? to_f32<T>(tokraw[j]) : 0.f;
-    float lowest = tok[0], highest = tok[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) {
-      lowest = min_nan(lowest, tok[j]);
-      highest = max_nan(highest, tok[j]);
-    }
-#pragma unroll
-    for (int s = 1; s < GS / 8; s <<= 1) {
-      lowest = min_nan(lowest, __shfl_xor_sync(0xffffffffu, lowest, s));
-      highest = max_nan(highest, __shfl_xor_sync(0xffffffffu, highest, s));
-    }
-    float step, lo, inverse;
-    q4_params(lowest, highest, step, lo, inverse);
-    tok_params = q4_pack_params(step, lo);
-    tok_codes = q4_codes(tok, step, lo, inverse);
-    if (tok_c < DK && ht == 0) {
-      uint8_t* out = (tok_value ? ring.v_codes : ring.k_codes) + (base + own) * C::CODES;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        out[(tok_value ? q4_value_place(DK, tok_c + 2 * j) : q4_key_place(DK, tok_c + 2 * j)) / 2] = (uint8_t)(tok_codes >> (8 * j));
-      if (tok_c % GS == 0) (tok_value ? ring.v_params : ring.k_params)[(base + own) * NG + tok_c / GS] = tok_params;
-    }
-    if (unit == 0 && lane == 0) ring.pos[b * SLOTS + own] = p;
-  }
-
-  float acc[TILES][4], low[NG][2], ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < TILES; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-#pragma unroll
-  for (int a = 0; a < NG; ++a) low[a][0] = low[a][1] = 0.f;
-  // row r of a 16-slot step is slot r, pairs swapped in the upper half of each eight: keys and values are then both
-  // read from shared memory without bank conflicts at DK 64
-  const int krow = g ^ ((g >> 2) & 1), vrow0 = (2 * t) ^ (t >> 1), vrow1 = (2 * t + 1) ^ (t >> 1);
-
-  for (int i = 0; lo_t + warp + AW * i < hi_t; ++i) {
-    const int tile = lo_t + warp + AW * i;
-    uint8_t* at = mine + (i % C::STAGES) * C::TILE;
-    cp_async_wait<C::STAGES - 1>();
-    __syncwarp();
-    if (has_own && own_at == warp + AW * i) {  // the token takes its slot here too
-      if (tok_c < DK) {
-        const int slot = own % TS;
-        uint8_t* codes = at + (tok_value ? C::VC : 0) + slot * C::CODES;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          codes[(tok_value ? q4_value_place(DK, tok_c + 2 * j) : q4_key_place(DK, tok_c + 2 * j)) / 2] =
-              (uint8_t)(tok_codes >> (8 * j));
-        if (tok_c % GS == 0)
-          reinterpret_cast<uint32_t*>(at + (tok_value ? C::VP : C::KP))[slot * NG + tok_c / GS] = tok_params;
-      }
-      __syncwarp();
-    }
-    // which of the slots are seen
-    uint32_t seen[TS / 32];
-#pragma unroll
-    for (int j = 0; j < TS / 32; ++j) {
-      const int slot = tile * TS + 32 * j + lane;
-      const int64_t kp = reinterpret_cast<const int64_t*>(at + C::POS)[32 * j + lane];
-      seen[j] = __ballot_sync(0xffffffffu, slot == own || (slot < W && kp >= 0 && (uint64_t)(p - kp) < (uint64_t)W));
-    }
-    bool every = true;
-#pragma unroll
-    for (int j = 0; j < TS / 32; ++j) every &= seen[j] == 0xffffffffu;
-    if (!every) {  // a slot that is not seen has step and lo 0, whatever it holds
-#pragma unroll
-      for (int x = 0; x < TS * NG / 32; ++x) {
-        const int slot = (32 * x + lane) / NG;
-        if (!((seen[slot >> 5] >> (slot & 31)) & 1u)) {
-          reinterpret_cast<uint32_t*>(at + C::KP)[32 * x + lane] = 0;
-          reinterpret_cast<uint32_t*>(at + C::VP)[32 * x + lane] = 0;
-        }
-      }
-      __syncwarp();
-    }
-    // scores of slots (rows) by heads (columns), to be multiplied by f
-    float s[MT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int r0 = 16 * mt + krow;
-      uint32_t c0[(DK / 8 + 3) / 4], c1[(DK / 8 + 3) / 4], p0[NG], p1[NG];
-      load_bytes<DK / 8>(at + r0 * C::CODES + t * (DK / 8), c0);
-      load_bytes<DK / 8>(at + (r0 + 8) * C::CODES + t * (DK / 8), c1);
-      load_bytes<4 * NG>(at + C::KP + r0 * C::PAR, p0);
-      load_bytes<4 * NG>(at + C::KP + (r0 + 8) * C::PAR, p1);
-      float tot[4] = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (C::LO_MMA) {
-        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at + C::KP + r0 * C::PAR + 4 * (t % NG));
-        const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + C::KP + (r0 + 8) * C::PAR + 4 * (t % NG));
-        mma_bf16_first(tot, w0, w1, w0, w1, qlo[0], qlo[1]);
-      } else {
-#pragma unroll
-        for (int a = 0; a < NG; ++a) {
-          // with codes as code - 7.5, lo + 7.5 step takes the place of lo
-          const float lo0 = C::EXACT ? fmaf(7.5f, q4_step(p0[a]), q4_lo(p0[a])) : q4_lo(p0[a]);
-          const float lo1 = C::EXACT ? fmaf(7.5f, q4_step(p1[a]), q4_lo(p1[a])) : q4_lo(p1[a]);
-          tot[0] = fmaf(lo0, qs[a][0], tot[0]);
-          tot[1] = fmaf(lo0, qs[a][1], tot[1]);
-          tot[2] = fmaf(lo1, qs[a][0], tot[2]);
-          tot[3] = fmaf(lo1, qs[a][1], tot[3]);
-        }
-      }
+        for (int i = 0; i < GS / 4; ++i) top = fmaxf(top, fabsf(x[a][i]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the power of two that brings the largest magnitude to [2^14, 2^15), and its inverse over the products' unit
+      const int e = top > 0.f ? (int)(__float_as_uint(top) >> 23) : 127;
+      const float up = __uint_as_float((uint32_t)min(268 - e, 254) << 23);
+      constexpr float UNIT = C::EXACT ? 1.f : 5.9604644775390625e-8f;  // what a product's code counts: 2^-24 in f16
+      const float down = ldexpf(1.0f, (C::EXACT ? 0 : 24) - (min(268 - e, 254) - 127));
 #pragma unroll
       for (int a = 0; a < NG; ++a) {
-        float d[4];
-        uint32_t w0, w1;
-        if constexpr (GS == 32) {
-          w0 = c0[a]; w1 = c1[a];
-        } else {  // four codes: the upper two in the upper half
-          w0 = (c0[a / 2] >> (16 * (a & 1))) & 0xffffu;
-          w1 = (c1[a / 2] >> (16 * (a & 1))) & 0xffffu;
-          w0 |= w0 << 8;
-          w1 |= w1 << 8;
-        }
+        sum[a] = 0.f;
 #pragma unroll
-        for (int k = 0; k < KSTEPS; ++k) {
-          const uint32_t x0 = w0 >> (8 * k), x1 = w1 >> (8 * k);
+        for (int i = 0; i < GS / 4; ++i) {
+          x[a][i] *= up;
+          sum[a] += x[a][i];
+        }
+        sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 1);
+        sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 2);
+        // nibbles (i, i + half) share a register: halves of a word of eight codes, or of four for groups of 16
+        constexpr int HALF = GS / 8;
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s) {
+          float u[4] = {x[a][2 * s], x[a][2 * s + HALF], x[a][2 * s + 1], x[a][2 * s + 1 + HALF]};
           if constexpr (C::EXACT) {
-            const uint32_t a0 = centred(x0), a1 = centred(x1), a2 = centred(x0 >> 4), a3 = centred(x1 >> 4);
 #pragma unroll
             for (int r = 0; r < QT; ++r) {
-              if (k == 0 && r == 0) mma_bf16_first(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
-              else mma_bf16(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+              qb[a][s][r][0] = pack_bf16(u[0], u[1]);
+              qb[a][s][r][1] = pack_bf16(u[2], u[3]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) u[i] -= __bfloat162float(__float2bfloat16_rn(u[i]));
             }
           } else {
-            const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
-            if (k == 0) mma_f16_first(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
-            else mma_f16(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
+            qb[a][s][0][0] = pack_f16(u[0], u[1]);
+            qb[a][s][0][1] = pack_f16(u[2] * 0.0625f, u[3] * 0.0625f);
           }
         }
-        const float s0 = q4_step(p0[a]), s1 = q4_step(p1[a]);
-        tot[0] = fmaf(s0, d[0], tot[0]);
-        tot[1] = fmaf(s0, d[1], tot[1]);
-        tot[2] = fmaf(s1, d[2], tot[2]);
-        tot[3] = fmaf(s1, d[3], tot[3]);
+      }
+      if constexpr (C::LO_MMA) {
+        // k = 2 t holds a step (times zero), k = 2 t + 1 the lo of group t, times the group's query sum in two terms
+        float mine_sum = 0.f;
+#pragma unroll
+        for (int a = 0; a < NG; ++a) mine_sum = t == a ? sum[a] * UNIT : mine_sum;
+        const float hi = __bfloat162float(__float2bfloat16_rn(mine_sum));
+        qlo[0] = pack_bf16(0.f, hi);
+        qlo[1] = pack_bf16(0.f, mine_sum - hi);
+      }
+      // what the sums' layout needs: heads 2 t and 2 t + 1
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int from = 4 * (2 * t + c);
+        f[c] = scale_log2 * __shfl_sync(0xffffffffu, down, from);
+#pragma unroll
+        for (int a = 0; a < NG; ++a) qs[a][c] = __shfl_sync(0xffffffffu, sum[a], from) * UNIT;
+      }
+    }
+
+    uint32_t tok_codes = 0, tok_params = 0;
+    if (has_own) {  // quantised, and written to the ring once per key head
+      float tok[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) tok[j] = tok_c < DK ? to_f32<T>(tokraw[j]) : 0.f;
+      float lowest = tok[0], highest = tok[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) {
+        lowest = min_nan(lowest, tok[j]);
+        highest = max_nan(highest, tok[j]);
       }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[mt][x] = tot[x];
+      for (int s = 1; s < GS / 8; s <<= 1) {
+        lowest = min_nan(lowest, __shfl_xor_sync(0xffffffffu, lowest, s));
+        highest = max_nan(highest, __shfl_xor_sync(0xffffffffu, highest, s));
+      }
+      float step, lo, inverse;
+      q4_params(lowest, highest, step, lo, inverse);
+      tok_params = q4_pack_params(step, lo);
+      tok_codes = q4_codes(tok, step, lo, inverse);
+      if (tok_c < DK && ht == 0) {
+        uint8_t* out = (tok_value ? ring.v_codes : ring.k_codes) + (base + own) * C::CODES;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          out[(tok_value ? q4_value_place(DK, tok_c + 2 * j) : q4_key_place(DK, tok_c + 2 * j)) / 2] = (uint8_t)(tok_codes >> (8 * j));
+        if (tok_c % GS == 0) (tok_value ? ring.v_params : ring.k_params)[(base + own) * NG + tok_c / GS] = tok_params;
+      }
+      if (unit == 0 && lane == 0) ring.pos[b * SLOTS + own] = p;
     }
-    if (!every) {
+
+    float acc[TILES][4], low[NG][2], ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+#pragma unroll
+    for (int a = 0; a < NG; ++a) low[a][0] = low[a][1] = 0.f;
+    // row r of a 16-slot step is slot r, pairs swapped in the upper half of each eight: keys and values are then both
+    // read from shared memory without bank conflicts at DK 64
+    const int krow = g ^ ((g >> 2) & 1), vrow0 = (2 * t) ^ (t >> 1), vrow1 = (2 * t + 1) ^ (t >> 1);
+
+    for (int i = 0; lo_t + warp + AW * i < hi_t; ++i) {
+      const int tile = lo_t + warp + AW * i;
+      uint8_t* at = mine + (i % C::STAGES) * C::TILE;
+      cp_async_wait<C::STAGES - 1>();
+      __syncwarp();
+      if (has_own && own_at == warp + AW * i) {  // the token takes its slot here too
+        if (tok_c < DK) {
+          const int slot = own % TS;
+          uint8_t* codes = at + (tok_value ? C::VC : 0) + slot * C::CODES;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            codes[(tok_value ? q4_value_place(DK, tok_c + 2 * j) : q4_key_place(DK, tok_c + 2 * j)) / 2] =
+                (uint8_t)(tok_codes >> (8 * j));
+          if (tok_c % GS == 0)
+            reinterpret_cast<uint32_t*>(at + (tok_value ? C::VP : C::KP))[slot * NG + tok_c / GS] = tok_params;
+        }
+        __syncwarp();
+      }
+      // which of the slots are seen
+      uint32_t seen[TS / 32];
+#pragma unroll
+      for (int j = 0; j < TS / 32; ++j) {
+        const int slot = tile * TS + 32 * j + lane;
+        const int64_t kp = reinterpret_cast<const int64_t*>(at + C::POS)[32 * j + lane];
+        seen[j] = __ballot_sync(0xffffffffu, slot == own || (slot < W && kp >= 0 && (uint64_t)(p - kp) < (uint64_t)W));
+      }
+      bool every = true;
+#pragma unroll
+      for (int j = 0; j < TS / 32; ++j) every &= seen[j] == 0xffffffffu;
+      if (!every) {  // a slot that is not seen has step and lo 0, whatever it holds
+#pragma unroll
+        for (int x = 0; x < TS * NG / 32; ++x) {
+          const int slot = (32 * x + lane) / NG;
+          if (!((seen[slot >> 5] >> (slot & 31)) & 1u)) {
+            reinterpret_cast<uint32_t*>(at + C::KP)[32 * x + lane] = 0;
+            reinterpret_cast<uint32_t*>(at + C::VP)[32 * x + lane] = 0;
+          }
+        }
+        __syncwarp();
+      }
+      // scores of slots (rows) by heads (columns), to be multiplied by f
+      float s[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const uint32_t bits = seen[mt >> 1] >> (16 * (mt & 1) + krow);
-        if (!(bits & 1u)) s[mt][0] = s[mt][1] = -INFINITY;
-        if (!(bits & 256u)) s[mt][2] = s[mt][3] = -INFINITY;
-      }
-    }
-    // the references, the weights and their sum
-    {
-      uint32_t big = 0;
+        const int r0 = 16 * mt + krow;
+        uint32_t c0[(DK / 8 + 3) / 4], c1[(DK / 8 + 3) / 4], p0[NG], p1[NG];
+        load_bytes<DK / 8>(at + r0 * C::CODES + t * (DK / 8), c0);
+        load_bytes<DK / 8>(at + (r0 + 8) * C::CODES + t * (DK / 8), c1);
+        load_bytes<4 * NG>(at + C::KP + r0 * C::PAR, p0);
+        load_bytes<4 * NG>(at + C::KP + (r0 + 8) * C::PAR, p1);
+        float tot[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (C::LO_MMA) {
+          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at + C::KP + r0 * C::PAR + 4 * (t % NG));
+          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + C::KP + (r0 + 8) * C::PAR + 4 * (t % NG));
+          mma_bf16_first(tot, w0, w1, w0, w1, qlo[0], qlo[1]);
+        } else {
 #pragma unroll
-      for (int x = 0; x < TS * NG / 32; ++x) big = max_bf16x2(big, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane]);
-      big = __reduce_max_sync(0xffffffffu, big << 16);  // the largest step, below 2^size
-      const float size = (float)max((int)(big >> 23) - 126, -104);
-      float top[2];
-      bool rise = false;
+          for (int a = 0; a < NG; ++a) {
+            // with codes as code - 7.5, lo + 7.5 step takes the place of lo
+            const float lo0 = C::EXACT ? fmaf(7.5f, q4_step(p0[a]), q4_lo(p0[a])) : q4_lo(p0[a]);
+            const float lo1 = C::EXACT ? fmaf(7.5f, q4_step(p1[a]), q4_lo(p1[a])) : q4_lo(p1[a]);
+            tot[0] = fmaf(lo0, qs[a][0], tot[0]);
+            tot[1] = fmaf(lo0, qs[a][1], tot[1]);
+            tot[2] = fmaf(lo1, qs[a][0], tot[2]);
+            tot[3] = fmaf(lo1, qs[a][1], tot[3]);
+          }
+        }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        top[c] = -INFINITY;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) top[c] = fmaxf(top[c], fmaxf(s[mt][c], s[mt][2 + c]));
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
-        top[c] = fmaf(top[c], f[c], size);
-        rise |= top[c] > ref[c] + 14.f;
-      }
-      if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float next = fmaxf(ref[c], top[c] - 6.f);
-          const float fade = next == -INFINITY ? 1.f : exp2_approx(ref[c] - next);
-          ref[c] = next;
-          l[c] *= fade;
-#pragma unroll
-          for (int j = 0; j < TILES; ++j) {
-            acc[j][c] *= fade;
-            acc[j][2 + c] *= fade;
+        for (int a = 0; a < NG; ++a) {
+          float d[4];
+          uint32_t w0, w1;
+          if constexpr (GS == 32) {
+            w0 = c0[a]; w1 = c1[a];
+          } else {  // four codes: the upper two in the upper half
+            w0 = (c0[a / 2] >> (16 * (a & 1))) & 0xffffu;
+            w1 = (c1[a / 2] >> (16 * (a & 1))) & 0xffffu;
+            w0 |= w0 << 8;
+            w1 |= w1 << 8;
           }
 #pragma unroll
-          for (int a = 0; a < NG; ++a) low[a][c] *= fade;
-        }
-      }
+          for (int k = 0; k < KSTEPS; ++k) {
+            const uint32_t x0 = w0 >> (8 * k), x1 = w1 >> (8 * k);
+            if constexpr (C::EXACT) {
+              const uint32_t a0 = centred(x0), a1 = centred(x1), a2 = centred(x0 >> 4), a3 = centred(x1 >> 4);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float r = ref[c] == -INFINITY ? 0.f : ref[c];
+              for (int r = 0; r < QT; ++r) {
+                if (k == 0 && r == 0) mma_bf16_first(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+                else mma_bf16(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+              }
+            } else {
+              const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+              if (k == 0) mma_f16_first(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
+              else mma_f16(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
+            }
+          }
+          const float s0 = q4_step(p0[a]), s1 = q4_step(p1[a]);
+          tot[0] = fmaf(s0, d[0], tot[0]);
+          tot[1] = fmaf(s0, d[1], tot[1]);
+          tot[2] = fmaf(s1, d[2], tot[2]);
+          tot[3] = fmaf(s1, d[3], tot[3]);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[mt][x] = tot[x];
+      }
+      if (!every) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          s[mt][c] = exp2_approx(fmaf(s[mt][c], f[c], -r));
-          s[mt][2 + c] = exp2_approx(fmaf(s[mt][2 + c], f[c], -r));
-          l[c] += s[mt][c] + s[mt][2 + c];
+          const uint32_t bits = seen[mt >> 1] >> (16 * (mt & 1) + krow);
+          if (!(bits & 1u)) s[mt][0] = s[mt][1] = -INFINITY;
+          if (!(bits & 256u)) s[mt][2] = s[mt][3] = -INFINITY;
         }
       }
-    }
-    // weights x values
+      // the references, the weights and their sum
+      {
+        uint32_t big = 0;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      constexpr int VB = DK / 16, VW = (VB + 3) / 4;
-      const int r0 = 16 * mt + krow;
-      uint32_t p0[NG], p1[NG], w[4][VW];
-      load_bytes<4 * NG>(at + C::VP + r0 * C::PAR, p0);
-      load_bytes<4 * NG>(at + C::VP + (r0 + 8) * C::PAR, p1);
-      const uint8_t* vc = at + C::VC + 16 * mt * C::CODES + g * VB;
-      load_bytes<VB>(vc + vrow0 * C::CODES, w[0]);
-      load_bytes<VB>(vc + vrow1 * C::CODES, w[1]);
-      load_bytes<VB>(vc + (vrow0 + 8) * C::CODES, w[2]);
-      load_bytes<VB>(vc + (vrow1 + 8) * C::CODES, w[3]);
+        for (int x = 0; x < TS * NG / 32; ++x) big = max_bf16x2(big, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane]);
+        big = __reduce_max_sync(0xffffffffu, big << 16);  // the largest step, below 2^size
+        // without any step the weights may be large, but not so large that a later tile's rescaling would lose them
+        const float size = big == 0 ? -40.f : (float)max((int)(big >> 23) - 126, -104);
+        float top[2];
+        bool rise = false;
 #pragma unroll
-      for (int a = 0; a < NG; ++a) {
-        const float st0 = q4_step(p0[a]), st1 = q4_step(p1[a]);
-        // with codes as code - 7.5, lo + 7.5 step takes the place of lo
-        const float lo0 = PT > 1 ? fmaf(7.5f, st0, q4_lo(p0[a])) : q4_lo(p0[a]);
-        const float lo1 = PT > 1 ? fmaf(7.5f, st1, q4_lo(p1[a])) : q4_lo(p1[a]);
-        low[a][0] = fmaf(s[mt][0], lo0, fmaf(s[mt][2], lo1, low[a][0]));
-        low[a][1] = fmaf(s[mt][1], lo0, fmaf(s[mt][3], lo1, low[a][1]));
-        float e[4] = {s[mt][0] * st0, s[mt][1] * st0, s[mt][2] * st1, s[mt][3] * st1};
-        uint32_t b0[PT], b1[PT];
+        for (int c = 0; c < 2; ++c) {
+          top[c] = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < PT; ++r) {
-          const uint32_t e0 = PT > 1 ? pack_bf16(e[0], e[1]) : pack_f16(e[0], e[1]);
-          const uint32_t e1 = PT > 1 ? pack_bf16(e[2], e[3]) : pack_f16(e[2], e[3]);
-          b0[r] = transpose8(e0);
-          b1[r] = transpose8(e1);
-          if constexpr (PT > 1) {
-            e[0] -= __uint_as_float(e0 << 16); e[1] -= __uint_as_float(e0 & 0xffff0000u);
-            e[2] -= __uint_as_float(e1 << 16); e[3] -= __uint_as_float(e1 & 0xffff0000u);
+          for (int mt = 0; mt < MT; ++mt) top[c] = fmaxf(top[c], fmaxf(s[mt][c], s[mt][2 + c]));
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
+          top[c] = fmaf(top[c], f[c], size);
+          rise |= top[c] > ref[c] + 14.f;
+        }
+        if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float next = fmaxf(ref[c], top[c] - 6.f);
+            const float fade = next == -INFINITY ? 1.f : exp2_approx(ref[c] - next);
+            ref[c] = next;
+            l[c] *= fade;
+#pragma unroll
+            for (int j = 0; j < TILES; ++j) {
+              acc[j][c] *= fade;
+              acc[j][2 + c] *= fade;
+            }
+#pragma unroll
+            for (int a = 0; a < NG; ++a) low[a][c] *= fade;
           }
         }
 #pragma unroll
-        for (int j = 0; j < GS / 16; ++j) {
-          const int i16 = a * (GS / 16) + j;  // channels [16 i16, 16 i16 + 16): byte i16 of the lanes' parts
-          const uint32_t sel = 0x4400u + 0x1111u * (i16 % 4);
-          // that byte of two slots in the low bytes of the halves: low four bits for rows g, the others for rows g + 8
-          const uint32_t x = __byte_perm(w[0][i16 / 4], w[1][i16 / 4], sel);
-          const uint32_t y = __byte_perm(w[2][i16 / 4], w[3][i16 / 4], sel);
-          if constexpr (PT > 1) {
-            const uint32_t a0 = centred(x), a1 = centred(x >> 4), a2 = centred(y), a3 = centred(y >> 4);
-            // the matrix unit's sums are cut off, not rounded: a short one, then a rounded addition
-            float d[4];
-            mma_bf16_first(d, a0, a1, a2, a3, b0[0], b1[0]);
+        for (int c = 0; c < 2; ++c) {
+          const float r = ref[c] == -INFINITY ? 0.f : ref[c];
 #pragma unroll
-            for (int r = 1; r < PT; ++r) mma_bf16(d, a0, a1, a2, a3, b0[r], b1[r]);
-#pragma unroll
-            for (int e2 = 0; e2 < 4; ++e2) acc[i16][e2] += d[e2];
-          } else {
-            mma_f16(acc[i16], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, b0[0], b1[0]);
+          for (int mt = 0; mt < MT; ++mt) {
+            s[mt][c] = exp2_approx(fmaf(s[mt][c], f[c], -r));
+            s[mt][2 + c] = exp2_approx(fmaf(s[mt][2 + c], f[c], -r));
+            l[c] += s[mt][c] + s[mt][2 + c];
           }
         }
       }
+      // weights x values
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        constexpr int VB = DK / 16, VW = (VB + 3) / 4;
+        const int r0 = 16 * mt + krow;
+        uint32_t p0[NG], p1[NG], w[4][VW];
+        load_bytes<4 * NG>(at + C::VP + r0 * C::PAR, p0);
+        load_bytes<4 * NG>(at + C::VP + (r0 + 8) * C::PAR, p1);
+        const uint8_t* vc = at + C::VC + 16 * mt * C::CODES + g * VB;
+        load_bytes<VB>(vc + vrow0 * C::CODES, w[0]);
+        load_bytes<VB>(vc + vrow1 * C::CODES, w[1]);
+        load_bytes<VB>(vc + (vrow0 + 8) * C::CODES, w[2]);
+        load_bytes<VB>(vc + (vrow1 + 8) * C::CODES, w[3]);
+#pragma unroll
+        for (int a = 0; a < NG; ++a) {
+          const float st0 = q4_step(p0[a]), st1 = q4_step(p1[a]);
+          // with codes as code - 7.5, lo + 7.5 step takes the place of lo
+          const float lo0 = PT > 1 ? fmaf(7.5f, st0, q4_lo(p0[a])) : q4_lo(p0[a]);
+          const float lo1 = PT > 1 ? fmaf(7.5f, st1, q4_lo(p1[a])) : q4_lo(p1[a]);
+          low[a][0] = fmaf(s[mt][0], lo0, fmaf(s[mt][2], lo1, low[a][0]));
+          low[a][1] = fmaf(s[mt][1], lo0, fmaf(s[mt][3], lo1, low[a][1]));
+          float e[4] = {s[mt][0] * st0, s[mt][1] * st0, s[mt][2] * st1, s[mt][3] * st1};
+          uint32_t b0[PT], b1[PT];
+#pragma unroll
+          for (int r = 0; r < PT; ++r) {
+            const uint32_t e0 = PT > 1 ? pack_bf16(e[0], e[1]) : pack_f16(e[0], e[1]);
+            const uint32_t e1 = PT > 1 ? pack_bf16(e[2], e[3]) : pack_f16(e[2], e[3]);
+            b0[r] = transpose8(e0);
+            b1[r] = transpose8(e1);
+            if constexpr (PT > 1) {
+              e[0] -= __uint_as_float(e0 << 16); e[1] -= __uint_as_float(e0 & 0xffff0000u);
+              e[2] -= __uint_as_float(e1 << 16); e[3] -= __uint_as_float(e1 & 0xffff0000u);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < GS / 16; ++j) {
+            const int i16 = a * (GS / 16) + j;  // channels [16 i16, 16 i16 + 16): byte i16 of the lanes' parts
+            const uint32_t sel = 0x4400u + 0x1111u * (i16 % 4);
+            // that byte of two slots in the low bytes of the halves: low four bits for rows g, the others for rows g + 8
+            const uint32_t x = __byte_perm(w[0][i16 / 4], w[1][i16 / 4], sel);
+            const uint32_t y = __byte_perm(w[2][i16 / 4], w[3][i16 / 4], sel);
+            if constexpr (PT > 1) {
+              const uint32_t a0 = centred(x), a1 = centred(x >> 4), a2 = centred(y), a3 = centred(y >> 4);
+              // the matrix unit's sums are cut off, not rounded: a short one, then a rounded addition
+              float d[4];
+              mma_bf16_first(d, a0, a1, a2, a3, b0[0], b1[0]);
+#pragma unroll
+              for (int r = 1; r < PT; ++r) mma_bf16(d, a0, a1, a2, a3, b0[r], b1[r]);
+#pragma unroll
+              for (int e2 = 0; e2 < 4; ++e2) acc[i16][e2] += d[e2];
+            } else {
+              mma_f16(acc[i16], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, b0[0], b1[0]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      copy(i + C::STAGES);
     }
-    __syncwarp();
-    copy(i + C::STAGES);
-  }
 
-  // this warp's part: heads 2 t and 2 t + 1, channels 16 i + 2 g and 16 i + 2 g + 1
-  cp_async_wait_all();  // also of copies that the position then made needless
-  __syncthreads();      // the stages are free
-  float* parts = reinterpret_cast<float*>(smem);  // [AW][HEADS][DK + 2]
+    // this warp's part: heads 2 t and 2 t + 1, channels 16 i + 2 g and 16 i + 2 g + 1
+    cp_async_wait_all();  // also of copies that the position then made needless
+    __syncthreads();      // the stages are free
+    float* parts = reinterpret_cast<float*>(smem);  // [AW][HEADS][DK + 2]
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < 2; ++c) {
 #pragma unroll
-    for (int x = 4; x < 32; x <<= 1) {
-      l[c] += __shfl_xor_sync(0xffffffffu, l[c], x);
+      for (int x = 4; x < 32; x <<= 1) {
+        l[c] += __shfl_xor_sync(0xffffffffu, l[c], x);
 #pragma unroll
-      for (int a = 0; a < NG; ++a) low[a][c] += __shfl_xor_sync(0xffffffffu, low[a][c], x);
-    }
-    float* row = parts + (warp * HEADS + 2 * t + c) * (DK + 2);
+        for (int a = 0; a < NG; ++a) low[a][c] += __shfl_xor_sync(0xffffffffu, low[a][c], x);
+      }
+      float* row = parts + (warp * HEADS + 2 * t + c) * (DK + 2);
 #pragma unroll
-    for (int i = 0; i < TILES; ++i) {
-      const int a = i / (GS / 16);
-      const float x = PT > 1 ? acc[i][c] : acc[i][c] * 16777216.f;        // f16: the codes' 2^-24
-      const float y = PT > 1 ? acc[i][2 + c] : acc[i][2 + c] * 1048576.f;  // and 2^-20
-      *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(x + low[a][c], y + low[a][c]);
-    }
-    if (g == 0) {
-      row[DK] = ref[c];
-      row[DK + 1] = l[c];
-    }
-  }
-  __syncthreads();
-  const bool whole = lo_t == 0 && hi_t == n;
-  if (shared && threadIdx.x == 0) {
-    if (lo_t == 0) span[b * units + unit].x = blockIdx.x;
-    if (hi_t == n) span[b * units + unit].y = blockIdx.x;
-  }
-  for (int e = threadIdx.x; e < heads * DK; e += AW * 32) {
-    const int h = e / DK, c = e - h * DK;
-    const float* col = parts + h * (DK + 2);
-    float M = -INFINITY, L = 0.f, out = 0.f;
-#pragma unroll
-    for (int w = 0; w < AW; ++w) M = fmaxf(M, col[w * HEADS * (DK + 2) + DK]);
-#pragma unroll
-    for (int w = 0; w < AW; ++w) {
-      const float* x = col + w * HEADS * (DK + 2);
-      const float fade = x[DK] == -INFINITY ? 0.f : exp2f(x[DK] - M);
-      L = fmaf(x[DK + 1], fade, L);
-      out = fmaf(x[c], fade, out);
-    }
-    if (whole) {
-      o[(b * H + h0 + h) * DK + c] = from_f32<T>(p < 0 ? 0.f : out / L);
-    } else {
-      float* to = part + (2 * (int64_t)blockIdx.x + (lo_t == 0)) * HEADS * (DK + 2) + h * (DK + 2);
-      to[c] = out;
-      if (c == 0) {
-        to[DK] = M;
-        to[DK + 1] = L;
+      for (int i = 0; i < TILES; ++i) {
+        const int a = i / (GS / 16);
+        const float x = PT > 1 ? acc[i][c] : acc[i][c] * 16777216.f;        // f16: the codes' 2^-24
+        const float y = PT > 1 ? acc[i][2 + c] : acc[i][2 + c] * 1048576.f;  // and 2^-20
+        *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(x + low[a][c], y + low[a][c]);
+      }
+      if (g == 0) {
+        row[DK] = ref[c];
+        row[DK + 1] = l[c];
       }
     }
-  }
-  if (from >= until) break;
-  // the next unit: its copies come into what was just read
-  __syncthreads();
-  if (hi_t == n && unit + 1 == units) {  // the next row that sees something
-    row_first += (int64_t)cost_of(n, opening) * units;
-    do n = tiles_of<TS>(pos[++b], W);
-    while (n == 0);
-  }
+    __syncthreads();
+    const bool whole = lo_t == 0 && hi_t == n;
+    if (shared && threadIdx.x == 0) {
+      if (lo_t == 0) span[b * units + unit].x = blockIdx.x;
+      if (hi_t == n) span[b * units + unit].y = blockIdx.x;
+    }
+    for (int e = threadIdx.x; e < heads * DK; e += AW * 32) {
+      const int h = e / DK, c = e - h * DK;
+      const float* col = parts + h * (DK + 2);
+      float M = -INFINITY, L = 0.f, out = 0.f;
+#pragma unroll
+      for (int w = 0; w < AW; ++w) M = fmaxf(M, col[w * HEADS * (DK + 2) + DK]);
+#pragma unroll
+      for (int w = 0; w < AW; ++w) {
+        const float* x = col + w * HEADS * (DK + 2);
+        const float fade = x[DK] == -INFINITY ? 0.f : exp2f(x[DK] - M);
+        L = fmaf(x[DK + 1], fade, L);
+        out = fmaf(x[c], fade, out);
+      }
+      if (whole) {
+        o[(b * H + h0 + h) * DK + c] = from_f32<T>(p < 0 ? 0.f : out / L);
+      } else {
+        float* to = part + (2 * (int64_t)blockIdx.x + (lo_t == 0)) * HEADS * (DK + 2) + h * (DK + 2);
+        to[c] = out;
+        if (c == 0) {
+          to[DK] = M;
+          to[DK + 1] = L;
+        }
+      }
+    }
+    if (from >= until) break;
+    // the next unit: its copies come into what was just read
+    __syncthreads();
+    if (hi_t == n && unit + 1 == units) {  // the next row that sees something
+      row_first += (int64_t)cost_of(n, opening) * units;
+      do n = tiles_of<TS>(pos[++b], W);
+      while (n == 0);
+    }
   }
 }
 

@@ -130,7 +130,11 @@ def _explain_ring(ring: Q4RingKVCache, what: str) -> tuple[int, int, int, int]:
 
 def _tokens(t: Tensor) -> Tensor:
     """``t [b, n, heads, dk]`` with each token's heads and channels dense, copied if they are not."""
-    dense = (t.stride(3) == 1 or t.shape[3] == 1) and (t.stride(2) == t.shape[3] or t.shape[2] == 1)
+    if t.is_contiguous():
+        return t
+    _, _, heads, dk = t.shape
+    _, _, head, channel = t.stride()
+    dense = (channel == 1 or dk == 1) and (head == dk or heads == 1)
     return t if dense else t.contiguous()
 
 
@@ -142,9 +146,10 @@ def _ring_ptrs(ring: Q4RingKVCache) -> tuple[int, int, int, int, int]:
 def _check_tokens(ring: Q4RingKVCache, k: Tensor, v: Tensor, pos: Tensor, what: str) -> tuple[int, int, int, int, int]:
     b, hkv, dk, slots = _check_ring(ring, what)
     device = ring.pos.device
+    shape = k.shape
     if not (
-        k.dim() == 4 and k.shape[0] == b and k.shape[2] == hkv and k.shape[3] == dk and v.shape == k.shape
-        and pos.shape == k.shape[:2] and pos.dtype == torch.int64 and k.dtype in SUPPORTED and v.dtype == k.dtype
+        len(shape) == 4 and shape[0] == b and shape[2] == hkv and shape[3] == dk and v.shape == shape
+        and pos.shape == shape[:2] and pos.dtype == torch.int64 and k.dtype in SUPPORTED and v.dtype == k.dtype
         and k.device == device and v.device == device and pos.device == device
     ):  # fmt: skip
         dims: Dims = {"b": b, "hkv": hkv, "dk": dk}
@@ -156,7 +161,7 @@ def _check_tokens(ring: Q4RingKVCache, k: Tensor, v: Tensor, pos: Tensor, what: 
             raise ContractError(msg)
         require_cuda(what, ring.pos, k=k, v=v, positions=pos)
     serving_only(what, k, v)
-    return b, k.shape[1], hkv, dk, slots
+    return b, shape[1], hkv, dk, slots
 
 
 @lru_cache(maxsize=256)
@@ -196,20 +201,22 @@ def q4_read(ring: Q4RingKVCache, pos: Tensor, dtype: torch.dtype = torch.bfloat1
         ContractError: on a shape, dtype or device mismatch, or a ring that is not dense.
     """
     b, hkv, dk, slots = _check_ring(ring, "4-bit cache")
-    dims: Dims = {"b": b}
-    check_shape("pos", pos, ("b", "n"), dims, torch.long)
-    require_cuda("4-bit cache", ring.pos, positions=pos)
-    if dtype not in SUPPORTED:
+    device = ring.pos.device
+    if not (
+        pos.dim() == 2 and pos.shape[0] == b and pos.dtype == torch.int64 and pos.device == device and dtype in SUPPORTED
+    ):  # fmt: skip
+        check_shape("pos", pos, ("b", "n"), {"b": b}, torch.long)
+        require_cuda("4-bit cache", ring.pos, positions=pos)
         msg = f"dtype: must be one of {SUPPORTED}, got {dtype}"
         raise ContractError(msg)
-    n = dims["n"]
-    k = torch.empty(b, n, hkv, dk, dtype=dtype, device=pos.device)
+    n = pos.shape[1]
+    k = torch.empty(b, n, hkv, dk, dtype=dtype, device=device)
     v = torch.empty_like(k)
-    held = torch.empty(b, n, dtype=torch.bool, device=pos.device)
+    held = torch.empty_like(pos, dtype=torch.bool, memory_format=torch.contiguous_format)
     if b and n:
         _lib.call(
             "vb_q4_read", *_ring_ptrs(ring), pos.contiguous().data_ptr(), k.data_ptr(), v.data_ptr(), held.data_ptr(),
-            b, n, hkv, dk, ring.window, slots, _lib.DTYPE_CODE[dtype], _lib.stream(pos.device),
+            b, n, hkv, dk, ring.window, slots, _lib.DTYPE_CODE[dtype], _lib.stream(device),
         )  # fmt: skip
     return k, v, held
 
@@ -227,31 +234,31 @@ def q4_attend_(q: Tensor, k: Tensor, v: Tensor, pos: Tensor, ring: Q4RingKVCache
             the key heads, or a ring that is not dense.
     """
     b, n, hkv, dk, slots = _check_tokens(ring, k, v, pos, "4-bit ring attention")
-    dims: Dims = {"b": b, "one": 1, "dk": dk}
     if not (q.dim() == 4 and q.shape[0] == b and q.shape[1] == 1 and q.shape[3] == dk):
-        check_shape("q", q, ("b", "one", "h", "dk"), dims)
+        check_shape("q", q, ("b", "one", "h", "dk"), {"b": b, "one": 1, "dk": dk})
     if n != 1:
         msg = f"k: axis 1 must be 1, got {n} (one token per row)"
         raise ContractError(msg)
     heads = q.shape[2]
-    if heads < 1 or heads % hkv != 0:
+    if hkv < 1 or heads < 1 or heads % hkv != 0:
         msg = f"{heads} query heads are not a multiple of {hkv} key heads"
         raise ContractError(msg)
     if q.dtype != k.dtype:
         msg = f"k: dtype must be {q.dtype} (q's), got {k.dtype}"
         raise ContractError(msg)
-    if q.device != k.device:
+    device = q.device
+    if device != k.device:
         require_cuda("4-bit ring attention", ring.pos, q=q)
     serving_only("4-bit ring attention", q)
-    o = torch.empty(b, 1, heads, dk, dtype=q.dtype, device=q.device)
+    o = torch.empty(b, 1, heads, dk, dtype=q.dtype, device=device)
     if b == 0:
         return o
     q, k, v, pos = _tokens(q), _tokens(k), _tokens(v), pos.contiguous()
     nbytes = _attend_workspace(b, heads, hkv, dk, ring.window)
-    ws = _lib.workspace(nbytes, q.device) if nbytes else None
+    ws = _lib.workspace(nbytes, device) if nbytes else None
     _lib.call(
         "vb_q4_attend", q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
         pos.data_ptr(), *_ring_ptrs(ring), o.data_ptr(), _lib.ptr(ws), b, heads, hkv, dk, ring.window, slots,
-        _lib.DTYPE_CODE[q.dtype], _lib.stream(q.device),
+        _lib.DTYPE_CODE[q.dtype], _lib.stream(device),
     )  # fmt: skip
     return o
