@@ -123,6 +123,22 @@ def test_rows_of_extreme_values(width: int) -> None:
     assert int(q[6, -1].abs()) == 127 and int(q[6].abs().sum()) == 127
 
 
+@pytest.mark.parametrize("width", [96, 4096, 5001])
+def test_norm_weights_at_the_ends_of_float32(width: int) -> None:
+    """Rows of one spike, whose norm is sqrt(width) times the weight there: no infinite factor and no infinite scale."""
+    x = torch.zeros(5, width)
+    x[:, 3] = torch.tensor([2.0, -2.0, 5.0, 1.0, 3.0])
+    for gain, zero, bad in ((1e-36, True, False), (1e-30, False, False), (2e38, False, True)):
+        q, scale = rms_norm_q8(x.to(CUDA), torch.full((width,), gain, device=CUDA), FLOOR, EPS)
+        if bad:  # the norm itself is infinite
+            assert bool(torch.isnan(scale).all()) and not bool(q.any())
+            continue
+        spike = x[:, 3].double().abs()
+        want = spike / torch.sqrt(spike.square() / width + EPS) * gain / 127
+        assert torch.equal(q[:, 3].cpu(), torch.tensor([0, 0, 0, 0, 0] if zero else [127, -127, 127, 127, 127], dtype=torch.int8))
+        assert bool((scale == 0).all() if zero else ((scale.cpu().double() - want).abs() <= 4e-6 * want).all())
+
+
 @pytest.mark.parametrize("relu_square", [False, True])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", [(1, 1), (64, 1536), (5, 17), (3, 4, 100), (40, 4097), (3, 20000)])
