@@ -7,12 +7,15 @@
 // linear_q8_split_kernel: few tokens. The weights' rows (output channels) lie on the accumulator's lanes and the
 //   tokens on its columns, so one token costs a tile of 16 columns. A cluster of S CTAs per tile of 128
 //   channels x BN tokens, each over its part of K; the parts are added through distributed shared memory, whole
-//   numbers, so the order does not matter. The weights are read once and that bounds it: S spreads their bytes over
-//   the SMs.
+//   numbers, so the order does not matter. The weights are read once, and S spreads their bytes over the SMs: 1 x 4096 x
+//   8192 in 8.7 us, 3.9 TB/s (59 % of a plain copy's rate; half the rest is the copies' start, the products' end and
+//   the clusters' sum). Small weights are bound by those alone: 64 x 512 x 1544 in 4.1 us.
 // linear_q8_tile_kernel: many tokens, on the lanes; persistent over tiles of 128 tokens x BN channels, or of 256 x 256
 //   on CTA pairs (cta_group::2), each CTA copying half of either operand (32 KB per 128 bytes of K, against 48 KB for
 //   a single CTA's 128 x 256). Accumulators are double-buffered in TMEM, so that the storing warps' loads,
-//   scaling and TMA stores run under the next tile's products.
+//   scaling and TMA stores run under the next tile's products. 8192 x 4096 x 8192 in 184 us, 2.98 POP/s, the tensor
+//   pipe active 75 % of the time (before the pairs 236 us, before the doubled accumulators 271); 777 x 1040 x 2001,
+//   91 tiles of nine blocks of K on 148 SMs, in 8.4 us: the latency of one tile.
 #include <cmath>
 
 #include "launch.cuh"
@@ -62,6 +65,8 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -127,6 +132,7 @@ __global__ void __launch_bounds__(128, 2)
   __shared__ float sxs[BN], sws[ROWS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = S > 1 ? (int)cluster_rank() : 0;
+  if (S > 1) cluster_arrive();
   const int n0 = (int)(blockIdx.x / S) * ROWS, m0 = blockIdx.y * BN;
   const int k_lo = (int)((int64_t)kblocks * rank / S), blocks = (int)((int64_t)kblocks * (rank + 1) / S) - k_lo;
   auto load = [&](int i) {
@@ -152,7 +158,6 @@ __global__ void __launch_bounds__(128, 2)
     tmem_relinquish();
   }
   grid_wait();
-  grid_release();
   if (tid >= 64)
     for (int i = tid - 64; i < BN + ROWS; i += 64) {
       if (i < BN) sxs[i] = m0 + i < M ? xs[m0 + i] : 0.f;
@@ -161,6 +166,7 @@ __global__ void __launch_bounds__(128, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_release();  // the next kernel comes once this one has its tensor memory
   const uint32_t tmem = tmem_at;
   if (tid == 0) {
     for (int i = C::STAGES; i < blocks; ++i) {
@@ -192,6 +198,8 @@ __global__ void __launch_bounds__(128, 2)
   __syncwarp();
   if (!mbar_wait(&done, 0)) gave_up(status);
   tc_fence_after();
+  __syncwarp();
+  if (S > 1) cluster_wait();  // the others have begun: their shared memory may be written
   // rank r adds and stores the channels [128 r / S, 128 (r + 1) / S): each CTA sends it their sums, in
   // pieces of four columns of one channel, [sender][column / 4][channel]
   const int per = ROWS / S, row = warp * 32 + lane, owner = row / per;
@@ -523,10 +531,10 @@ int sm_count() {
 template <int BN, typename T>
 int launch_split(const Args& a) {
   const int kblocks = (a.K + KB - 1) / KB, tiles_n = (a.N + ROWS - 1) / ROWS, tiles_m = (a.M + BN - 1) / BN;
-  // K over S CTAs: one per SM, or two where each still has four blocks of K to itself (1 x 4096 x 8192: 9.1 us with
-  // two, 10.8 with one; 64 x 512 x 1544, whose CTAs would be left one block: 5.5 with two, 5.0 with one)
+  // K over S CTAs: one per SM, or two where each still has two blocks of K to itself (1 x 4096 x 8192: 8.7 us with
+  // two, 10.1 with one; 1 x 1024 x 8192: 4.9 and 5.4; 1 x 1024 x 4096, whose CTAs would be left one block: 5.0 and 4.3)
   int S = 1;
-  while (S < 8 && 2 * S <= kblocks && 2LL * S * tiles_n * tiles_m <= (long long)sm_count() * (kblocks / (2 * S) >= 4 ? 2 : 1))
+  while (S < 8 && 2 * S <= kblocks && 2LL * S * tiles_n * tiles_m <= (long long)sm_count() * (kblocks / (2 * S) >= 2 ? 2 : 1))
     S *= 2;
   CUtensorMap wmap, xmap;
   int rc = make_byte_map(&wmap, a.wq, a.N, a.K, a.ldw, ROWS);
@@ -573,14 +581,15 @@ extern "C" int vb_linear_q8(const int8_t* xq, int64_t ldx, const float* xs, cons
   const Args a{xq, ldx, xs, wq, ldw, ws, y, M, N, K, status, (cudaStream_t)stream};
   return VB_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     // Few tokens: the split kernel, whose time is the weights' bytes. Tiles of 32 tokens rather than 64 where the
-    // weights are small and CTAs few (64 x 1536 x 512: 5.0 us against 5.7; 64 x 4096 x 8192: 14.2 against 11.2).
+    // weights are small and CTAs few (64 x 1536 x 512: 4.2 us against 4.7; 64 x 4096 x 8192: 12.9 against 10.8). Up to
+    // 256 tokens while K is long (256 x 4096 x 4096: 12.1 us, in tiles 13.7; 256 x 512 x 1544: 6.0 and 4.2).
     const int64_t kb = (K + KB - 1) / KB;
     if (M <= 16) return launch_split<16, T>(a);
     if (M <= 32 || (M <= 64 && (int64_t)N * K <= (4 << 20))) return launch_split<32, T>(a);
     if (M <= 64 || (M <= 256 && kb > 16)) return launch_split<64, T>(a);
     // Else the tile that the measured times of one wave favour, in tenths of a microsecond per wave of tiles: the
-    // larger of its products' time per block of K and its store's. 1024 x 4096 x 4096: 17.5 us on pairs, 26.9 with
-    // 128 channels, 46 with 64; 4096 x 512 x 1536: 11.3, 9.0, 13.1; 1024 x 1024 x 1024: 9.0, 6.8, 6.4.
+    // larger of its products' time per block of K and its store's. 1024 x 4096 x 4096: 17.0 us on pairs, 25.5 with
+    // 128 channels, 45.4 with 64; 4096 x 512 x 1536: 9.3, 8.6, 12.4; 1024 x 1024 x 1024: 7.7, 6.1, 5.6.
     const int sms = sm_count();
     auto waves = [&](int tm, int tn, int slots) { return ((int64_t)((M + tm - 1) / tm) * ((N + tn - 1) / tn) + slots - 1) / slots; };
     const double pair = 40 + waves(256, 256, sms / 2) * fmax(4.1 * kb, 34.0);

@@ -44,10 +44,11 @@ def serving_only(what: str, *tensors: Tensor) -> None:
 
 def _codes(x: Tensor) -> tuple[Tensor, Tensor, int]:
     """Empty codes and scales for ``x``'s rows, and the codes' row pitch."""
-    lead, width, device = x.shape[:-1], x.shape[-1], x.device
-    scale = torch.empty(lead, dtype=torch.float32, device=device)
+    *lead, width = x.shape
+    device = x.device
+    scale = torch.empty(*lead, dtype=torch.float32, device=device) if lead else torch.empty((), dtype=torch.float32, device=device)
     if width % 16 == 0:
-        return torch.empty(x.shape, dtype=torch.int8, device=device), scale, width
+        return torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format), scale, width
     pitch = -(-width // 16) * 16
     return torch.empty(*lead, pitch, dtype=torch.int8, device=device)[..., :width], scale, pitch
 
@@ -160,13 +161,14 @@ def quantize_rows_q8(x: Tensor, *, relu_square: bool = False) -> tuple[Tensor, T
 def _pitched(t: Tensor) -> tuple[Tensor, int]:
     """``t [rows, K]`` int8 with rows a multiple of 16 bytes apart from a 16-byte boundary, and their
     pitch: ``t`` itself where it is laid out so (as this module's codes are), else a copy."""
-    k = t.shape[-1]
-    if t.stride(1) == 1 or k == 1:
-        pitch = t.stride(0) if t.shape[0] > 1 else -(-k // 16) * 16
+    n, k = t.shape
+    row, step = t.stride()
+    if step == 1 or k == 1:
+        pitch = row if n > 1 else -(-k // 16) * 16
         if pitch % 16 == 0 and pitch >= k and t.data_ptr() % 16 == 0:
             return t, pitch
     pitch = -(-k // 16) * 16
-    copy = torch.zeros(t.shape[0], pitch, dtype=torch.int8, device=t.device)
+    copy = torch.zeros(n, pitch, dtype=torch.int8, device=t.device)
     copy[:, :k] = t
     return copy, pitch
 
@@ -200,7 +202,7 @@ def dequantize_rows_q8(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.floa
         if (width > 1 and flat.stride(1) != 1) or (rows > 1 and flat.stride(0) < width):
             flat = flat.contiguous()
         pitch = flat.stride(0) if rows > 1 else width
-    y = torch.empty(q.shape, dtype=dtype, device=q.device)
+    y = torch.empty(*q.shape, dtype=dtype, device=q.device)
     _lib.call(
         "vb_dequantize_rows_q8", flat.data_ptr(), pitch, scale.contiguous().data_ptr(), y.data_ptr(), rows, width,
         _lib.DTYPE_CODE[dtype], _lib.stream(q.device),
@@ -210,14 +212,15 @@ def dequantize_rows_q8(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.floa
 
 def _check_linear(xq: Tensor, xs: Tensor, wq: Tensor, ws: Tensor, out_dtype: torch.dtype) -> tuple[int, int]:
     """``(N, K)``: accepts in one expression what is well-formed, else finds out what is not."""
-    device = xq.device
-    if (
-        wq.dim() == 2 and xq.dim() >= 1 and wq.dtype == torch.int8 == xq.dtype and xs.dtype == torch.float32 == ws.dtype
-        and 1 <= wq.shape[1] <= MAX_K and wq.shape[0] <= MAX_ROWS and xs.numel() <= MAX_ROWS and xq.shape[-1] == wq.shape[1] and xs.shape == xq.shape[:-1]
-        and ws.shape == wq.shape[:1] and wq.shape[0] >= 1 and out_dtype in SUPPORTED and xq.is_cuda
-        and xs.device == device and wq.device == device and ws.device == device
-    ):  # fmt: skip
-        return wq.shape[0], wq.shape[1]
+    if wq.dim() == 2 and xq.dim() >= 1:
+        device, x_shape, (n, k) = xq.device, xq.shape, wq.shape
+        if (
+            wq.dtype == torch.int8 == xq.dtype and xs.dtype == torch.float32 == ws.dtype
+            and 1 <= k <= MAX_K and 1 <= n <= MAX_ROWS and xs.numel() <= MAX_ROWS and x_shape[-1] == k
+            and xs.shape == x_shape[:-1] and ws.shape == (n,) and out_dtype in SUPPORTED and xq.is_cuda
+            and xs.device == device and wq.device == device and ws.device == device
+        ):  # fmt: skip
+            return n, k
     dims: Dims = {}
     check_shape("wq", wq, ("N", "K"), dims, torch.int8)
     check_shape("ws", ws, ("N",), dims, torch.float32)
@@ -249,14 +252,15 @@ def linear_q8(xq: Tensor, xs: Tensor, wq: Tensor, ws: Tensor, out_dtype: torch.d
             of int8 products may leave int32).
     """
     n, k = _check_linear(xq, xs, wq, ws, out_dtype)
+    device = xq.device
     flat = xq if xq.dim() == 2 else xq.reshape(-1, k)
     rows, ldx = _pitched(flat)
     weights, ldw = _pitched(wq)
-    m = flat.shape[0]
-    y = torch.empty(*xq.shape[:-1], n, dtype=out_dtype, device=xq.device)
+    m = xs.numel()
+    y = torch.empty(m, n, dtype=out_dtype, device=device)
     _lib.call(
         "vb_linear_q8", rows.data_ptr(), ldx, xs.contiguous().data_ptr(), weights.data_ptr(), ldw,
         ws.contiguous().data_ptr(), y.data_ptr(), m, n, k, _lib.DTYPE_CODE[out_dtype],
-        _lib.status_word(xq.device).data_ptr(), _lib.stream(xq.device),
+        _lib.status_word(device).data_ptr(), _lib.stream(device),
     )  # fmt: skip
-    return y
+    return y if flat is xq else y.view(*xq.shape[:-1], n)
