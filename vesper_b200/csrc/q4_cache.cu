@@ -3,7 +3,11 @@
 // The format is q4.cuh's. A CTA takes some tokens of one (row, key head) (32 at DK 128), keys and values: a thread per
 // eight channels (16 bytes of bf16), a group's extremes by shuffles among its neighbours, and the
 // codes by way of shared memory, where they find their places a byte or a word at a time and leave or arrive in
-// 8-byte pieces of consecutive slots. HBM bound: 2 bytes in and 0.625 out per bf16 channel.
+// 8-byte pieces of consecutive slots. HBM bound by their bytes (2 in and 0.625 out per bf16 channel, or the reverse), in
+// practice by the instructions between: 4 x 32701 tokens, 8 heads of 128, are written in 175 us (4.0 TB/s, 61 % of a plain
+// copy's rate; instructions issue in 83 % of the cycles) and read back in 151 us (4.7 TB/s, 71 %; 70 %). float32 tokens,
+// with twice the bytes for each, are written at 5.9 TB/s (90 %). 64 x 2048 tokens into a window of 512, one head of 64:
+// 7.1 and 6.1 us.
 #include <type_traits>
 
 #include "launch.cuh"
@@ -259,8 +263,8 @@ int check_ring(const char* what, int B, int N, int HKV, int DK, int W, int SLOTS
   VB_REQUIRE(SLOTS % Q4_TILE == 0 && SLOTS >= W, "%s: %d slots must be a multiple of %d holding the window %d", what,
              SLOTS, Q4_TILE, W);
   VB_REQUIRE(dtype_size(dtype) > 0, "%s: unsupported dtype code %d", what, dtype);
-  VB_REQUIRE(B <= 65535 && HKV <= 65535 && (int64_t)N * HKV < (int64_t(1) << 31), "%s: %d rows of %d tokens x %d key heads exceed the grid",
-             what, B, N, HKV);
+  VB_REQUIRE(B <= 65535 && HKV <= 65535 && (int64_t)N * HKV < (int64_t(1) << 31),
+             "%s: %d rows of %d tokens x %d key heads exceed the grid", what, B, N, HKV);
   return VB_OK;
 }
 
@@ -300,8 +304,9 @@ extern "C" int vb_q4_write(void* k_codes, void* k_params, void* v_codes, void* v
                   v_batch * size % 16 == 0 && v_token * size % 16 == 0;
   return VB_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return with_head_dim(DK, [&](auto dk) -> int {
-      return launch_early("q4_write", q4_write_kernel<T, decltype(dk)::value>, dim3((min(N, W) + Layout<decltype(dk)::value>::ROWS - 1) / Layout<decltype(dk)::value>::ROWS, HKV, B), NT,
-                          0, 1, (cudaStream_t)stream, ring, (const T*)k, k_batch, k_token, (const T*)v, v_batch, v_token, pos,
+      constexpr int D = decltype(dk)::value, ROWS = Layout<D>::ROWS;
+      return launch_early("q4_write", q4_write_kernel<T, D>, dim3((min(N, W) + ROWS - 1) / ROWS, HKV, B), NT, 0, 1,
+                          (cudaStream_t)stream, ring, (const T*)k, k_batch, k_token, (const T*)v, v_batch, v_token, pos,
                           vec, N, HKV, W, SLOTS);
     });
   });
@@ -320,7 +325,8 @@ extern "C" int vb_q4_read(const void* k_codes, const void* k_params, const void*
              "q4_read: the buffers must start on 16-byte boundaries");
   return VB_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return with_head_dim(DK, [&](auto dk) -> int {
-      return launch_early("q4_read", q4_read_kernel<T, decltype(dk)::value>, dim3((N + Layout<decltype(dk)::value>::ROWS - 1) / Layout<decltype(dk)::value>::ROWS * HKV, B), NT, 0, 1,
+      constexpr int D = decltype(dk)::value, ROWS = Layout<D>::ROWS;
+      return launch_early("q4_read", q4_read_kernel<T, D>, dim3((N + ROWS - 1) / ROWS * HKV, B), NT, 0, 1,
                           (cudaStream_t)stream, ring, pos, (T*)k, (T*)v, held, N, HKV, W, SLOTS);
     });
   });
