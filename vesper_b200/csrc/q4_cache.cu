@@ -1,13 +1,12 @@
 // The 4-bit ring cache: tokens quantised as they are written, and read back at given positions
 // (a RingKVCache, vesper/attention.py:63-139, whose keys and values take five bits a channel).
-// The format is q4.cuh's. A CTA takes some tokens of one (row, key head) (32 at DK 128), keys and values: a thread per
-// eight channels (16 bytes of bf16), a group's extremes by shuffles among its neighbours, and the
-// codes by way of shared memory, where they find their places a byte or a word at a time and leave or arrive in
-// 8-byte pieces of consecutive slots. HBM bound by their bytes (2 in and 0.625 out per bf16 channel, or the reverse), in
-// practice by the instructions between: 4 x 32701 tokens, 8 heads of 128, are written in 175 us (4.0 TB/s, 61 % of a plain
-// copy's rate; instructions issue in 83 % of the cycles) and read back in 151 us (4.7 TB/s, 71 %; 70 %). float32 tokens,
-// with twice the bytes for each, are written at 5.9 TB/s (90 %). 64 x 2048 tokens into a window of 512, one head of 64:
-// 7.1 and 6.1 us.
+// The format is q4.cuh's. A CTA takes some tokens of one (row, key head) (16 at DK 128), keys and values: a group's
+// extremes from a thread's registers and its neighbour's, and the codes by way of shared memory, where they find their
+// places a byte or a word at a time and leave or arrive in 8-byte pieces of consecutive slots. HBM bound: 2 bytes in and
+// 0.625 out per bf16 channel, or the reverse. 4 x 32701 tokens, 8 heads of 128, are written in 144 us (4.9 TB/s, 75 % of
+// a plain copy's rate; the instructions are near as many as the cycles) and read back in 148 us (4.75 TB/s, 73 %: 3.6
+// TB/s of stores, as much as filling memory reaches). float32 tokens, with twice the bytes for each, are written at 6.1
+// TB/s (93 %). 64 x 2048 tokens into a window of 512, one head of 64: 6.3 and 6.0 us.
 #include <type_traits>
 
 #include "launch.cuh"
@@ -16,15 +15,21 @@
 namespace vb {
 namespace {
 
-constexpr int NT = 256;
+constexpr int NT = 128;  // more and smaller CTAs start and end in turn (with 256, read back: 4 x 32701 tokens of 8 heads of 128
+                         // 151 us against 148, 4 x 16384 of 8 heads of 64 in float32 61 against 55)
 
-// how a CTA's threads lie over its tokens: a thread per eight channels, two passes; then a thread per 8 bytes of codes and
-// per group's parameters
+// How a CTA's threads lie over its tokens. Writing: a thread per sixteen channels of a group, in two pieces of eight half a
+// group apart, so that half of a group's work is a thread's own and two neighbours read 32 bytes of bf16 at a time (4 x
+// 32701 tokens, 8 heads of 128: 144 us, with a thread per eight channels 175). Reading: a thread per eight channels, two
+// passes over the tokens, whose float32 stores cover whole lines (4 x 16384 tokens of 8 heads of 64: 61 us, in two
+// pieces 75). For codes a thread per 8 bytes, for parameters a thread per group.
 template <int DK>
 struct Layout {
-  static constexpr int PER = DK / 8, RP = NT / PER, ROWS = 2 * RP;  // threads per token, tokens per pass and per CTA
   static constexpr int GS = q4_group(DK), NG = DK / GS, HALF = DK / 2;
-  static_assert(ROWS * (HALF / 8) <= NT && ROWS * NG <= NT, "one step each");
+  static constexpr int PER = DK / 16, ROWS = NT / PER;             // writing: threads per token, tokens per CTA
+  static constexpr int GL = GS / 16, PIECE = GS / 2;               // threads per group, from one piece to the other
+  static constexpr int PER8 = DK / 8, PASS = NT / PER8, READ_ROWS = 2 * PASS;  // reading
+  static_assert(ROWS * (HALF / 8) <= NT && ROWS * NG <= NT && READ_ROWS <= ROWS, "one step each");
 };
 
 struct Q4Ring {
@@ -55,28 +60,32 @@ struct __align__(16) Raw8 {
   }
 };
 
-// the smallest and the largest of eight elements, NaN if one is; 16-bit types two at a time
-__device__ __forceinline__ void extremes(const Raw8<float>& raw, float& low, float& high) {
-  low = high = raw.v[0];
+// the smallest and the largest of sixteen elements, NaN if one is; 16-bit types two at a time
+__device__ __forceinline__ void extremes(const Raw8<float> (&raw)[2], float& low, float& high) {
+  low = high = raw[0].v[0];
 #pragma unroll
-  for (int e = 1; e < 8; ++e) {
-    low = min_nan(low, raw.v[e]);
-    high = max_nan(high, raw.v[e]);
+  for (int e = 1; e < 16; ++e) {
+    low = min_nan(low, raw[e / 8].v[e % 8]);
+    high = max_nan(high, raw[e / 8].v[e % 8]);
   }
 }
-__device__ __forceinline__ void extremes(const Raw8<__nv_bfloat16>& raw, float& low, float& high) {
-  const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(raw.v);
-  const __nv_bfloat162 l = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
-  const __nv_bfloat162 h = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+template <typename T2, typename T>
+__device__ __forceinline__ void extremes2(const Raw8<T> (&raw)[2], float& low, float& high) {
+  const T2 *w = reinterpret_cast<const T2*>(raw[0].v), *u = reinterpret_cast<const T2*>(raw[1].v);
+  T2 l = __hmin2_nan(w[0], u[0]), h = __hmax2_nan(w[0], u[0]);
+#pragma unroll
+  for (int e = 1; e < 4; ++e) {
+    l = __hmin2_nan(l, __hmin2_nan(w[e], u[e]));
+    h = __hmax2_nan(h, __hmax2_nan(w[e], u[e]));
+  }
   low = min_nan(__low2float(l), __high2float(l));
   high = max_nan(__low2float(h), __high2float(h));
 }
-__device__ __forceinline__ void extremes(const Raw8<__half>& raw, float& low, float& high) {
-  const __half2* w = reinterpret_cast<const __half2*>(raw.v);
-  const __half2 l = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
-  const __half2 h = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
-  low = min_nan(__low2float(l), __high2float(l));
-  high = max_nan(__low2float(h), __high2float(h));
+__device__ __forceinline__ void extremes(const Raw8<__nv_bfloat16> (&raw)[2], float& low, float& high) {
+  extremes2<__nv_bfloat162>(raw, low, high);
+}
+__device__ __forceinline__ void extremes(const Raw8<__half> (&raw)[2], float& low, float& high) {
+  extremes2<__half2>(raw, low, high);
 }
 
 // Tokens [B, N] at positions pos, negative ones (padding, at either end of a row) not written. Of those that share a
@@ -87,33 +96,33 @@ __global__ void __launch_bounds__(NT) q4_write_kernel(Q4Ring ring, const T* __re
                                                       const int64_t* __restrict__ pos, int vec, int N, int HKV,
                                                       int W, int SLOTS) {
   using L = Layout<DK>;
-  constexpr int PER = L::PER, RP = L::RP, ROWS = L::ROWS, GS = L::GS, NG = L::NG, HALF = L::HALF;
+  constexpr int PER = L::PER, ROWS = L::ROWS, GS = L::GS, NG = L::NG, HALF = L::HALF, PIECE = L::PIECE;
   __shared__ __align__(16) uint8_t codes[2][ROWS][HALF];
   __shared__ uint32_t params[2][ROWS][NG];
   __shared__ int slots[ROWS];  // -1: not written
   // consecutive CTAs take consecutive tokens of a head, whose slots they fill side by side (4 x 32701 tokens, 8 heads of
-  // 128: 170 us; with a token's heads next to each other 186)
+  // 128: 144 us; with a token's heads next to each other 154)
   const int tid = threadIdx.x, block = blockIdx.x, kh = blockIdx.y;
   const int64_t b = blockIdx.z;
-  const int row0 = tid / PER, c0 = tid % PER * 8;
-  const bool busy = RP * PER == NT || tid < RP * PER;
+  const int mine = tid / PER, c0 = tid % PER / L::GL * GS + tid % PER % L::GL * 8;
+  const bool busy = ROWS * PER == NT || tid < ROWS * PER;
   grid_wait();
   grid_release();
   const int64_t* at = pos + b * N;
-  Raw8<T> raw[2][2];       // [keys, values][pass]
+  Raw8<T> raw[2][2];       // [keys, values][piece]
   int end = N, first = 0;  // the tokens before the padding at the row's end, and the first of this CTA's
   int64_t p = -1;
   auto fetch = [&] {  // every load of the thread in flight before any is used
     first = max(0, end - W) + block * ROWS;
     if (tid < ROWS && first + tid < end) p = at[first + tid];
-    const T* from[2] = {k + b * kb + (int64_t)(first + row0) * kt + (int64_t)kh * DK + c0,
-                        v + b * vb_ + (int64_t)(first + row0) * vt + (int64_t)kh * DK + c0};
+    if (!busy || first + mine >= end) return;
+    const T* from[2] = {k + b * kb + (int64_t)(first + mine) * kt + (int64_t)kh * DK + c0,
+                        v + b * vb_ + (int64_t)(first + mine) * vt + (int64_t)kh * DK + c0};
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (busy && first + row0 + i * RP < end) {
-        raw[0][i].load(from[0] + i * RP * kt, vec);
-        raw[1][i].load(from[1] + i * RP * vt, vec);
-      }
+    for (int i = 0; i < 2; ++i) {
+      raw[0][i].load(from[0] + i * PIECE, vec);
+      raw[1][i].load(from[1] + i * PIECE, vec);
+    }
   };
   fetch();  // as if there were no padding at the end
   if (at[N - 1] < 0) {
@@ -135,37 +144,46 @@ __global__ void __launch_bounds__(NT) q4_write_kernel(Q4Ring ring, const T* __re
     if (kh == 0 && p >= 0) ring.pos[b * SLOTS + slots[tid]] = p;
   }
 #pragma unroll
-  for (int value = 0; value < 2; ++value)
+  for (int value = 0; value < 2; ++value) {
+    // a token that is not written holds what it may here and is left out below
+    float x[2][8], low, high;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      // a token that is not written holds what it may here and is left out below
-      const int row = row0 + i * RP;
-      float x[8], low, high;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = to_f32<T>(raw[value][i].v[e]);
-      extremes(raw[value][i], low, high);
-      // the lanes of a group are neighbours (PER is a multiple of a group's lanes)
-#pragma unroll
-      for (int o = 1; o < GS / 8; o <<= 1) {
-        low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
-        high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
-      }
-      float step, lo, inverse;
-      q4_params(low, high, step, lo, inverse);
-      const uint32_t w = q4_codes(x, step, lo, inverse);
-      if (!busy) continue;
-      uint8_t* to = codes[value][row];
-      if (value) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) to[q4_value_place(DK, c0 + 2 * e) / 2] = (uint8_t)(w >> (8 * e));
-      } else if constexpr (GS == 32) {
-        *reinterpret_cast<uint32_t*>(to + q4_key_place(DK, c0) / 2) = w;
-      } else {
-        *reinterpret_cast<uint16_t*>(to + q4_key_place(DK, c0) / 2) = (uint16_t)w;
-        *reinterpret_cast<uint16_t*>(to + q4_key_place(DK, c0 + 4) / 2) = (uint16_t)(w >> 16);
-      }
-      if (c0 % GS == 0) params[value][row][c0 / GS] = q4_pack_params(step, lo);
+      for (int e = 0; e < 8; ++e) x[i][e] = to_f32<T>(raw[value][i].v[e]);
+    extremes(raw[value], low, high);
+    if constexpr (L::GL == 2) {  // the other half of the group: a neighbour's (PER is even)
+      low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, 1));
+      high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, 1));
     }
+    float step, lo, inverse;
+    q4_params(low, high, step, lo, inverse);
+    const uint32_t w0 = q4_codes(x[0], step, lo, inverse), w1 = q4_codes(x[1], step, lo, inverse);
+    if (!busy) continue;
+    uint8_t* to = codes[value][mine];
+    if (value && GS == 32) {  // the two pieces' codes are neighbours
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<uint16_t*>(to + q4_value_place(DK, c0 + 2 * e) / 2) =
+            (uint16_t)__byte_perm(w0, w1, e | (4 + e) << 4);
+    } else if (value) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        to[q4_value_place(DK, c0 + 2 * e) / 2] = (uint8_t)(w0 >> (8 * e));
+        to[q4_value_place(DK, c0 + PIECE + 2 * e) / 2] = (uint8_t)(w1 >> (8 * e));
+      }
+    } else if (GS == 32) {
+      *reinterpret_cast<uint32_t*>(to + q4_key_place(DK, c0) / 2) = w0;
+      *reinterpret_cast<uint32_t*>(to + q4_key_place(DK, c0 + PIECE) / 2) = w1;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        *reinterpret_cast<uint16_t*>(to + q4_key_place(DK, c0 + 4 * e) / 2) = (uint16_t)(w0 >> (16 * e));
+        *reinterpret_cast<uint16_t*>(to + q4_key_place(DK, c0 + PIECE + 4 * e) / 2) = (uint16_t)(w1 >> (16 * e));
+      }
+    }
+    if (c0 % GS == 0) params[value][mine][c0 / GS] = q4_pack_params(step, lo);
+  }
   __syncthreads();
   const int64_t base = (b * HKV + kh) * SLOTS;
   {
@@ -189,12 +207,13 @@ __global__ void __launch_bounds__(NT) q4_read_kernel(Q4Ring ring, const int64_t*
                                                      T* __restrict__ v, uint8_t* __restrict__ held, int N, int HKV,
                                                      int W, int SLOTS) {
   using L = Layout<DK>;
-  constexpr int PER = L::PER, RP = L::RP, ROWS = L::ROWS, GS = L::GS, NG = L::NG, HALF = L::HALF;
+  constexpr int PER = L::PER8, RP = L::PASS, ROWS = L::READ_ROWS, GS = L::GS, NG = L::NG, HALF = L::HALF;
   __shared__ __align__(16) uint8_t codes[2][ROWS][HALF];
   __shared__ uint32_t params[2][ROWS][NG];
   __shared__ int slots[ROWS];  // -1: no position that a ring could hold
   __shared__ bool have[ROWS];
-  // consecutive CTAs take the heads of the same tokens, whose values lie side by side (the same: 151 us; by head 157)
+  // consecutive CTAs take the heads of the same tokens, whose values lie side by side (the same, with 256 threads:
+  // 151 us; by head 157)
   const int tid = threadIdx.x, block = blockIdx.x / HKV, kh = blockIdx.x - block * HKV, first = block * ROWS;
   const int64_t b = blockIdx.y;
   grid_wait();
@@ -325,7 +344,7 @@ extern "C" int vb_q4_read(const void* k_codes, const void* k_params, const void*
              "q4_read: the buffers must start on 16-byte boundaries");
   return VB_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     return with_head_dim(DK, [&](auto dk) -> int {
-      constexpr int D = decltype(dk)::value, ROWS = Layout<D>::ROWS;
+      constexpr int D = decltype(dk)::value, ROWS = Layout<D>::READ_ROWS;
       return launch_early("q4_read", q4_read_kernel<T, D>, dim3((N + ROWS - 1) / ROWS * HKV, B), NT, 0, 1,
                           (cudaStream_t)stream, ring, pos, (T*)k, (T*)v, held, N, HKV, W, SLOTS);
     });
