@@ -288,6 +288,19 @@ def test_sharp_and_large_scores(dtype: torch.dtype) -> None:
     _check_attend(zero, 4, [99, 99], 77, dtype, scale=0.0)
 
 
+@pytest.mark.parametrize(("dk", "window"), [(64, 512), (128, 5000), (80, 3001)])
+def test_an_f16_output_is_off_by_little_more_than_its_own_rounding(dk: int, window: int) -> None:
+    """Rounding to f16 costs 2^-11 / sqrt(6) = 2.0e-4 of the norm (uniform errors, uniform mantissas); the float32 sums
+    and products in 22 bits leave room for half as much again."""
+    b, h, hkv = 3, 8, 2
+    ring = _filled(b, hkv, dk, window, [window] * b, 65, torch.float16)
+    q = torch.randn(b, 1, h, dk, generator=torch.Generator().manual_seed(66)).half().to(CUDA)
+    k, v = (t.to(CUDA) for t in _tokens(b, 1, hkv, dk, 67, torch.float16))
+    pos = torch.full((b, 1), window, device=CUDA)
+    o = q4_attend_(q, k, v, pos, ring)
+    assert rel(o.double().cpu().numpy(), _attend_want(ring, q, pos).numpy()) < 3e-4
+
+
 @pytest.mark.parametrize("size", [2.0**-20, 1.0, 2.0**40])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_tiles_of_constant_values_among_large_ones(dtype: torch.dtype, size: float) -> None:

@@ -13,8 +13,8 @@
 //     divided by 16 where their codes come 16-fold. The group's step and lo are applied to the float32 sums.
 //   output  O[channel, head] = sum_slot (w step) code + w lo: m16n8k16 in f16, channels as rows, the codes again as
 //     they are (those in the upper four bits make their rows of O 16-fold, taken off at the end). The products w step
-//     are rounded to f16 (2^-12 of each, of both signs), whose range they fit because the scores' reference is chosen
-//     with the largest step in view. They cross from the scores' layout to the operand's by movmatrix.
+//     are rounded to f16 (2^-12 of each, of both signs; for an f16 output in two terms), whose range they fit because the
+//     scores' reference is chosen with the largest step in view. They cross from the scores' layout to the operand's by movmatrix.
 // For float32 inputs queries and products are held in three bf16 terms and the codes as bf16 code - 7.5, around zero, and
 // the matrix unit's sums, which are cut off rather than rounded, are short: the output is within 1e-6 of its norm.
 // A reference r and the sum of the weights 2^(score - r) per warp and head in float32; r rises only when a weight
@@ -53,9 +53,12 @@ struct Q4Attn {
   static constexpr int TILE = POS + TS * 8;
   static constexpr int AW = 8, STAGES = 2, CTAS = ctas_per_sm(DK);  // warps per CTA, tiles in flight per warp
   static constexpr int SMEM = AW * STAGES * TILE;
-  // float32 throughout: queries and the weights' products in three bf16 terms, codes as code - 7.5; else one f16 term
+  // float32 throughout: queries and the weights' products in three bf16 terms, codes as code - 7.5. Else queries in one
+  // f16 term, which a 16-bit query is, and the products in one for a bf16 output (8 x 8192 positions, 32 / 8 heads of 128:
+  // 1.72e-3 off in all, the output's rounding alone 1.65e-3), in two for an f16 output, which would show their rounding
+  // (5.1e-4 with one in 28.0 us, 2.3e-4 with two in 31.1, its rounding alone 2.1e-4)
   static constexpr bool EXACT = sizeof(T) == 4;
-  static constexpr int QT = EXACT ? 3 : 1, PT = QT;
+  static constexpr int QT = EXACT ? 3 : 1, PT = EXACT ? 3 : std::is_same<T, __half>::value ? 2 : 1;
   // the sum of lo times the queries' sums as one product in bf16: four groups, two terms
   static constexpr bool LO_MMA = !EXACT && (NG == 1 || NG == 2 || NG == 4);
 };
@@ -624,19 +627,24 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         for (int a = 0; a < NG; ++a) {
           const float st0 = q4_step(p0[a]), st1 = q4_step(p1[a]);
           // with codes as code - 7.5, lo + 7.5 step takes the place of lo
-          const float lo0 = PT > 1 ? fmaf(7.5f, st0, q4_lo(p0[a])) : q4_lo(p0[a]);
-          const float lo1 = PT > 1 ? fmaf(7.5f, st1, q4_lo(p1[a])) : q4_lo(p1[a]);
+          const float lo0 = C::EXACT ? fmaf(7.5f, st0, q4_lo(p0[a])) : q4_lo(p0[a]);
+          const float lo1 = C::EXACT ? fmaf(7.5f, st1, q4_lo(p1[a])) : q4_lo(p1[a]);
           low[a][0] = fmaf(s[mt][0], lo0, fmaf(s[mt][2], lo1, low[a][0]));
           low[a][1] = fmaf(s[mt][1], lo0, fmaf(s[mt][3], lo1, low[a][1]));
           float e[4] = {s[mt][0] * st0, s[mt][1] * st0, s[mt][2] * st1, s[mt][3] * st1};
           uint32_t b0[PT], b1[PT];
 #pragma unroll
           for (int r = 0; r < PT; ++r) {
-            const uint32_t e0 = PT > 1 ? pack_bf16(e[0], e[1]) : pack_f16(e[0], e[1]);
-            const uint32_t e1 = PT > 1 ? pack_bf16(e[2], e[3]) : pack_f16(e[2], e[3]);
+            const uint32_t e0 = C::EXACT ? pack_bf16(e[0], e[1]) : pack_f16(e[0], e[1]);
+            const uint32_t e1 = C::EXACT ? pack_bf16(e[2], e[3]) : pack_f16(e[2], e[3]);
             b0[r] = transpose8(e0);
             b1[r] = transpose8(e1);
-            if constexpr (PT > 1) {
+            if constexpr (!C::EXACT && PT > 1) {
+              const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&e0));
+              const float2 r1 = __half22float2(*reinterpret_cast<const __half2*>(&e1));
+              e[0] -= r0.x; e[1] -= r0.y;
+              e[2] -= r1.x; e[3] -= r1.y;
+            } else if constexpr (C::EXACT) {
               e[0] -= __uint_as_float(e0 << 16); e[1] -= __uint_as_float(e0 & 0xffff0000u);
               e[2] -= __uint_as_float(e1 << 16); e[3] -= __uint_as_float(e1 & 0xffff0000u);
             }
@@ -648,7 +656,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
             // that byte of two slots in the low bytes of the halves: low four bits for rows g, the others for rows g + 8
             const uint32_t x = __byte_perm(w[0][i16 / 4], w[1][i16 / 4], sel);
             const uint32_t y = __byte_perm(w[2][i16 / 4], w[3][i16 / 4], sel);
-            if constexpr (PT > 1) {
+            if constexpr (C::EXACT) {
               const uint32_t a0 = centred(x), a1 = centred(x >> 4), a2 = centred(y), a3 = centred(y >> 4);
               // the matrix unit's sums are cut off, not rounded: a short one, then a rounded addition
               float d[4];
@@ -658,7 +666,9 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
 #pragma unroll
               for (int e2 = 0; e2 < 4; ++e2) acc[i16][e2] += d[e2];
             } else {
-              mma_f16(acc[i16], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, b0[0], b1[0]);
+              const uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+#pragma unroll
+              for (int r = 0; r < PT; ++r) mma_f16(acc[i16], a0, a1, a2, a3, b0[r], b1[r]);
             }
           }
         }
@@ -683,8 +693,8 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
         const int a = i / (GS / 16);
-        const float x = PT > 1 ? acc[i][c] : acc[i][c] * 16777216.f;        // f16: the codes' 2^-24
-        const float y = PT > 1 ? acc[i][2 + c] : acc[i][2 + c] * 1048576.f;  // and 2^-20
+        const float x = C::EXACT ? acc[i][c] : acc[i][c] * 16777216.f;        // f16: the codes' 2^-24
+        const float y = C::EXACT ? acc[i][2 + c] : acc[i][2 + c] * 1048576.f;  // and 2^-20
         *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(x + low[a][c], y + low[a][c]);
       }
       if (g == 0) {
