@@ -50,7 +50,11 @@ def _codes(x: Tensor) -> tuple[Tensor, Tensor, int]:
     if width % 16 == 0:
         return torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format), scale, width
     pitch = -(-width // 16) * 16
-    return torch.empty(*lead, pitch, dtype=torch.int8, device=device)[..., :width], scale, pitch
+    strides, step = [1], pitch
+    for n in reversed(lead):
+        strides.insert(0, step)
+        step *= n
+    return torch.empty_strided(x.shape, strides, dtype=torch.int8, device=device), scale, pitch
 
 
 def _check_norm(x: Tensor, r: Tensor | None, weight: Tensor) -> None:
@@ -198,7 +202,7 @@ def dequantize_rows_q8(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.floa
     if q.is_contiguous():
         flat, pitch = q, width
     else:
-        flat = q.reshape(rows, width)  # a view of codes as this module lays them out
+        flat = q if q.dim() == 2 else q.reshape(rows, width)  # a view of codes as this module lays them out
         if (width > 1 and flat.stride(1) != 1) or (rows > 1 and flat.stride(0) < width):
             flat = flat.contiguous()
         pitch = flat.stride(0) if rows > 1 else width
