@@ -27,8 +27,8 @@
 // latency: eight warps an SM (238 registers each at DK 128) issue in half of the cycles, and the last tiles of a unit, the
 // joining of its warps and the next unit's first tiles follow one another. At DK 64, eight query heads to two key heads,
 // 64 x 8192 take 30.3 us (88 MB, 44 %): half the bytes for each instruction. 64 rows of 512 positions take 5.2 us, the
-// latency of position, tiles, two products and the joining. One float32 row of 100003 positions at DK 64, its
-// products nine times over, takes 21 us.
+// latency of position, tiles, two products and the joining. One float32 row of 100003 positions at DK 64,
+// three products for one, takes 21 us.
 #include <cmath>
 #include <type_traits>
 
