@@ -316,6 +316,24 @@ def test_tiles_of_constant_values_among_large_ones(dtype: torch.dtype, size: flo
     _check_attend(ring, 4, [window - 1, window + 5], 79, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [2.0**12, 2.0**24, 2.0**60])
+def test_large_values_of_no_weight_do_not_touch_the_others(dtype: torch.dtype, size: float) -> None:
+    """Every 40th token has values ``size`` times larger and a key that no query attends (weights below e^-130)."""
+    b, hkv, h, dk, window = 2, 1, 4, 64, 700
+    g = torch.Generator().manual_seed(68)
+    k, v = _tokens(b, window, hkv, dk, 69, dtype)
+    u = torch.nn.functional.normalize(torch.randn(dk, generator=g), dim=0)
+    v[:, 7::40] = v[:, 7::40] * size
+    k[:, 7::40] = (-60 * u).to(dtype)
+    ring = q4_write_(q4_ring_empty(b, hkv, dk, window, CUDA), k.to(CUDA), v.to(CUDA), _positions([0, 0], window).to(CUDA))
+    q = (20 * u + torch.randn(b, 1, h, dk, generator=g)).to(dtype).to(CUDA)
+    t, w = (x.to(CUDA) for x in _tokens(b, 1, hkv, dk, 70, dtype))
+    pos = torch.full((b, 1), window, device=CUDA)
+    o = q4_attend_(q, t, w, pos, ring)
+    assert rel(o.double().cpu().numpy(), _attend_want(ring, q, pos).numpy()) < TOL[dtype]
+
+
 def test_strided_tokens_and_streams() -> None:
     b, h, hkv, dk = 4, 8, 2, 64
     ring1, ring2 = (_filled(b, hkv, dk, 96, [95, 96, 97, 10], 80, torch.bfloat16) for _ in range(2))

@@ -18,15 +18,16 @@
 // For float32 inputs queries and products are held in three bf16 terms and the codes as bf16 code - 7.5, around zero, and
 // the matrix unit's sums, which are cut off rather than rounded, are short: the output is within 1e-6 of its norm.
 // A reference r and the sum of the weights 2^(score - r) per warp and head in float32; r rises only when a weight
-// times the largest step of its tile would pass 2^14, and then to 2^6, so that the sums are seldom rescaled. The
-// warps' parts are joined in shared memory, those of the CTAs that share a long window by a second kernel, in a fixed
-// order. A slot that is not seen has score -inf and its step and lo are read as zeros, whatever it holds.
+// times its tile's largest step (its slot's, where steps lie far apart) would pass 2^14, and then to 2^6, so that the
+// sums are seldom rescaled. The warps' parts are joined in shared memory, those of the CTAs that share a long window by
+// a second kernel, in a fixed order. A slot that is not seen has score -inf and its step and lo are read as zeros,
+// whatever it holds.
 //
-// Measured (bf16, device): 8 rows of 6249 to 49999 positions, 32 query and 8 key heads of 128, 61.5 us (290 MB, 4.7
-// TB/s, 72 % of a plain copy's rate); 8 x 32768 69.7 us (4.85 TB/s, 74 %). What keeps it from the copy's rate is
+// Measured (bf16, device): 8 rows of 6249 to 49999 positions, 32 query and 8 key heads of 128, 62 us (290 MB, 4.7
+// TB/s, 71 % of a plain copy's rate); 8 x 32768 70 us (4.8 TB/s, 74 %). What keeps it from the copy's rate is
 // latency: eight warps an SM (238 registers each at DK 128) issue in half of the cycles, and the last tiles of a unit, the
 // joining of its warps and the next unit's first tiles follow one another. At DK 64, eight query heads to two key heads,
-// 64 x 8192 take 30.3 us (88 MB, 44 %): half the bytes for each instruction. 64 rows of 512 positions take 5.2 us, the
+// 64 x 8192 take 30.7 us (88 MB, 44 %): half the bytes for each instruction. 64 rows of 512 positions take 5.4 us, the
 // latency of position, tiles, two products and the joining. One float32 row of 100003 positions at DK 64,
 // three products for one, takes 21 us.
 #include <cmath>
@@ -143,6 +144,12 @@ __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t (&w)[(BYTE
 #pragma unroll
     for (int i = 0; i < BYTES; ++i) w[i / 4] |= (uint32_t)p[i] << (8 * (i & 3));
   }
+}
+
+// A power of two above a step (given as bits), as its exponent. Bounded below, where the weights' sum would leave float32;
+// and without any step the weights may be large, but not so large that a later tile's rescaling would lose them.
+__device__ __forceinline__ float size_of(uint32_t step) {
+  return step == 0 ? -40.f : (float)max((int)(step >> 23) - 126, -80);
 }
 
 struct Ring {
@@ -569,8 +576,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
 #pragma unroll
         for (int x = 0; x < TS * NG / 32; ++x) big = max_bf16x2(big, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane]);
         big = __reduce_max_sync(0xffffffffu, big << 16);  // the largest step, below 2^size
-        // without any step the weights may be large, but not so large that a later tile's rescaling would lose them
-        const float size = big == 0 ? -40.f : (float)max((int)(big >> 23) - 126, -104);
+        const float size = size_of(big);
         float top[2];
         bool rise = false;
 #pragma unroll
@@ -584,9 +590,32 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
           rise |= top[c] > ref[c] + 14.f;
         }
         if (__any_sync(0xffffffffu, rise)) {
+          uint32_t small = 0xffffffffu;
+#pragma unroll
+          for (int x = 0; x < TS * NG / 32; ++x)
+            small = min(small, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane] << 16);
+          if ((big >> 23) - (__reduce_min_sync(0xffffffffu, small) >> 23) > 8) {
+            // steps far apart: every slot with its own, so that large values of little weight take no precision from others
+            top[0] = top[1] = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 2 * MT; ++x) {
+              uint32_t par[NG];
+              load_bytes<4 * NG>(at + C::VP + (8 * x + krow) * C::PAR, par);
+              float step = 0.f;
+#pragma unroll
+              for (int a = 0; a < NG; ++a) step = fmaxf(step, q4_step(par[a]));
+              const float slot_size = size_of(__float_as_uint(step));
+#pragma unroll
+              for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], fmaf(s[x / 2][x % 2 * 2 + c], f[c], slot_size));
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
+          }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float next = fmaxf(ref[c], top[c] - 6.f);
+            const float next = top[c] > ref[c] + 14.f ? top[c] - 6.f : ref[c];
             const float fade = next == -INFINITY ? 1.f : exp2_approx(ref[c] - next);
             ref[c] = next;
             l[c] *= fade;
