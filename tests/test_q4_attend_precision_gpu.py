@@ -1,0 +1,65 @@
+"""What 4-bit ring attention (``q4_attend_``) keeps of 16-bit inputs, on a B200, against 64-bit arithmetic.
+
+Tolerances, derived before the first run:
+
+- rounding an output to f16 costs 2^-11 / sqrt(6) = 2.0e-4 of the norm (uniform errors, uniform mantissas); float32 sums, of
+  however many positions, leave room for half as much again: 3e-4.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from vesper_b200.kernels.q4_cache import Q4RingKVCache, q4_attend_, q4_read, q4_ring_empty, q4_write_
+
+pytestmark = pytest.mark.gpu
+CUDA = torch.device("cuda")
+
+
+def _want(ring: Q4RingKVCache, q: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
+    """A masked softmax in 64 bits over what the ring holds, the token among it."""
+    b, _, h, dk = q.shape
+    hkv, w = ring.k_codes.shape[1], ring.window
+    out = torch.zeros(b, 1, h, dk, dtype=torch.float64, device=CUDA)
+    for i in range(b):
+        p = int(pos[i])
+        if p < 0:
+            continue
+        one = Q4RingKVCache(*(getattr(ring, n)[i : i + 1] for n in ("k_codes", "k_params", "v_codes", "v_params", "pos")), w)
+        at = one.pos[:, :w]
+        k, v, held = q4_read(one, at, torch.float32)
+        seen = (held & (at <= p) & (at > p - w))[0]
+        qi = q[i, 0].double().view(hkv, h // hkv, dk)
+        wt = torch.softmax(torch.einsum("hgd,lhd->hgl", qi, k[0, seen].double()) / dk**0.5, -1)
+        out[i, 0] = torch.einsum("hgl,lhd->hgd", wt, v[0, seen].double()).reshape(h, dk)
+    return out
+
+
+def _full(b: int, hkv: int, dk: int, window: int, seed: int, dtype: torch.dtype) -> Q4RingKVCache:
+    """A ring that holds positions 0 .. window - 1 of normally distributed keys and values."""
+    g = torch.Generator(device=CUDA).manual_seed(seed)
+    ring = q4_ring_empty(b, hkv, dk, window, CUDA)
+    k, v = (torch.randn(b, window, hkv, dk, generator=g, device=CUDA).to(dtype) for _ in range(2))
+    return q4_write_(ring, k, v, torch.arange(window, device=CUDA).expand(b, window))
+
+
+def _step(b: int, h: int, hkv: int, dk: int, pos: list[int], seed: int, dtype: torch.dtype) -> tuple[torch.Tensor, ...]:
+    """A token's ``q``, ``k``, ``v`` and position."""
+    g = torch.Generator(device=CUDA).manual_seed(seed)
+    q, k, v = (torch.randn(b, 1, x, dk, generator=g, device=CUDA).to(dtype) for x in (h, hkv, hkv))
+    return q, k, v, torch.tensor(pos, device=CUDA)[:, None]
+
+
+def _rel(o: torch.Tensor, want: torch.Tensor) -> float:
+    return float((o.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize(("b", "h", "hkv", "dk", "window"), [(64, 2, 1, 16, 65536), (64, 4, 1, 64, 40000), (16, 7, 1, 128, 65536),
+                                                           (48, 5, 1, 48, 30000)])  # fmt: skip
+def test_long_sums_in_f16_are_float32_sums(b: int, h: int, hkv: int, dk: int, window: int) -> None:
+    """Dozens of tiles a warp, every weight of the same order: the outputs are small against the values they average."""
+    ring = _full(b, hkv, dk, window, 1, torch.float16)
+    q, k, v, pos = _step(b, h, hkv, dk, [window] * b, 2, torch.float16)
+    o = q4_attend_(q, k, v, pos, ring)
+    assert _rel(o, _want(ring, q, pos)) < 3e-4
