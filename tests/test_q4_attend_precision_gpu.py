@@ -3,7 +3,12 @@
 Tolerances, derived before the first run:
 
 - rounding an output to f16 costs 2^-11 / sqrt(6) = 2.0e-4 of the norm (uniform errors, uniform mantissas); float32 sums, of
-  however many positions, leave room for half as much again: 3e-4.
+  however many positions, leave room for half as much again: 3e-4;
+- a bf16 output is the float32 result rounded once. Float32 arithmetic leaves it within 1e-5 of the outputs' size (as for
+  float32 inputs), which moves an output x across a rounding boundary, 2^-8 |x| or more apart, with a probability
+  of at most 2 * 1e-5 * 2^8 / |x| (x in units of the outputs' size). Over normally distributed x that is 5e-3 E[min(1 / |x|,
+  200)] = 5e-3 * sqrt(2 / pi) * (ln 200 + 0.06) = 2.1 %. So at least 97.5 % of the outputs equal the 64-bit result
+  rounded to bf16.
 """
 
 from __future__ import annotations
@@ -63,3 +68,14 @@ def test_long_sums_in_f16_are_float32_sums(b: int, h: int, hkv: int, dk: int, wi
     q, k, v, pos = _step(b, h, hkv, dk, [window] * b, 2, torch.float16)
     o = q4_attend_(q, k, v, pos, ring)
     assert _rel(o, _want(ring, q, pos)) < 3e-4
+
+
+@pytest.mark.parametrize(("h", "hkv"), [(8, 2), (16, 2), (3, 1), (9, 1)])
+@pytest.mark.parametrize(("dk", "window"), [(64, 512), (128, 5000), (80, 3001), (16, 100)])
+def test_a_bf16_output_is_the_float32_result_rounded(dk: int, window: int, h: int, hkv: int) -> None:
+    b = 8
+    ring = _full(b, hkv, dk, window, 3, torch.bfloat16)
+    q, k, v, pos = _step(b, h, hkv, dk, [window] * b, 4, torch.bfloat16)
+    o = q4_attend_(q, k, v, pos, ring)
+    equal = float((o == _want(ring, q, pos).to(torch.bfloat16)).double().mean())
+    assert equal >= 0.975, equal

@@ -13,8 +13,8 @@
 //     divided by 16 where their codes come 16-fold. The group's step and lo are applied to the float32 sums.
 //   output  O[channel, head] = sum_slot (w step) code + w lo: m16n8k16 in f16, channels as rows, the codes again as
 //     they are (those in the upper four bits make their rows of O 16-fold, taken off at the end). The products w step
-//     are rounded to f16 (2^-12 of each, of both signs; for an f16 output in two terms), whose range they fit because the
-//     scores' reference is chosen with the largest step in view. They cross from the scores' layout to the operand's by movmatrix.
+//     are held in two f16 terms (22 bits), whose range they fit because the scores' reference is chosen with the largest
+//     step in view. They cross from the scores' layout to the operand's by movmatrix.
 //     The matrix unit cuts its sums off, always towards zero: with codes of one sign the loss of a long run would add up, to
 //     15 times an f16 output's rounding where a warp has 50 tiles of equal weights. So every second step of 16 slots takes
 //     15 - code (the complement, at no cost) with the products negated, and the sums stay near zero (1 to 2 % of the time).
@@ -58,11 +58,10 @@ struct Q4Attn {
   static constexpr int AW = 8, STAGES = 2, CTAS = ctas_per_sm(DK);  // warps per CTA, tiles in flight per warp
   static constexpr int SMEM = AW * STAGES * TILE;
   // float32 throughout: queries and the weights' products in three bf16 terms, codes as code - 7.5. Else queries in one
-  // f16 term, which a 16-bit query is, and the products in one for a bf16 output (8 x 8192 positions, 32 / 8 heads of 128:
-  // 1.72e-3 off in all, the output's rounding alone 1.65e-3), in two for an f16 output, which would show their rounding
-  // (5.1e-4 with one in 28.0 us, 2.3e-4 with two in 31.1, its rounding alone 2.1e-4)
+  // f16 term, which a 16-bit query is, and the products in two (with one, 17 % of a bf16 output's numbers are not the
+  // rounded result, with two 0.4 %)
   static constexpr bool EXACT = sizeof(T) == 4;
-  static constexpr int QT = EXACT ? 3 : 1, PT = EXACT ? 3 : std::is_same<T, __half>::value ? 2 : 1;
+  static constexpr int QT = EXACT ? 3 : 1, PT = EXACT ? 3 : 2;
   // the sum of lo times the queries' sums as one product in bf16: four groups, two terms
   static constexpr bool LO_MMA = !EXACT && (NG == 1 || NG == 2 || NG == 4);
 };
@@ -108,6 +107,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// x and y plus m (an f16 number, as bits) times the f16 numbers of a pair, in float32
+constexpr uint16_t F16_MINUS_ONE = 0xbc00;
+__device__ __forceinline__ void less_f16(float& x, float& y, uint32_t pair, uint16_t m) {
+  asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "fma.rn.f32.f16 %0, a, %3, %0;\n\tfma.rn.f32.f16 %1, b, %3, %1;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "r"(pair), "h"(m));
 }
 
 // the low four bits of each half as a pair of bf16 numbers code - 7.5: 16 + code by their place in the mantissa, less 23.5
@@ -245,7 +253,10 @@ struct Share {
 // not hold whole to its partials, [2 i] of the unit it starts within and [2 i + 1] of the one it ends within, each
 // [HEADS][DK + 2]: per head the unnormalised output, the reference and the sum; span[row][unit] gets the first and
 // the last CTA of a unit. Else a CTA per unit and row.
-template <typename T, int DK>
+// PAIR: at most four heads to a key head. Columns 4 to 7 of the products then repeat the heads of columns 0 to 3, bit for bit,
+// and take the second f16 term of the weights' products, so that two terms cost no second product (8 x 32768 positions, 32 /
+// 8 heads of 128: 75 us, with two products 82; a single term 72).
+template <typename T, int DK, bool PAIR>
 __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
     q4_attn_kernel(const T* __restrict__ q, int64_t q_row, int q_vec, const T* __restrict__ k_new, int64_t k_row,
                    const T* __restrict__ v_new, int64_t v_row, const int64_t* __restrict__ pos, Ring ring,
@@ -253,7 +264,8 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
                    int HKV, int head_tiles, int W, int SLOTS, float scale_log2) {
   using C = Q4Attn<T, DK>;
   constexpr int GS = C::GS, NG = C::NG, QT = C::QT, PT = C::PT, TILES = DK / 16, KSTEPS = GS / 16, AW = C::AW;
-  constexpr int TS = C::TS, MT = C::MT;
+  constexpr int TS = C::TS, MT = C::MT, PM = PAIR ? 1 : PT;  // PM: products for a step's terms
+  static_assert(!(PAIR && C::EXACT), "three terms do not fit two columns");
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int units = HKV * head_tiles, G = H / HKV;
@@ -289,11 +301,12 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
     }
     const int kh = unit / head_tiles, ht = unit - kh * head_tiles, h0 = kh * G + ht * HEADS, heads = min(HEADS, G - ht * HEADS);
     const int64_t base = (b * HKV + kh) * SLOTS;
+    const int column = PAIR ? g & 3 : g;  // the head whose query this thread holds
     // queries: thread (g, t) holds head g's channels of every group that the key codes of lane part t belong to. They and
     // the token are loaded before the cache's tiles, behind which they would wait
     __align__(16) T xraw[NG * (GS / 4)], tokraw[8];  // as they come: nothing waits for them before the copies are issued
     {
-      const T* src = q + b * q_row + (int64_t)(h0 + min(g, heads - 1)) * DK + t * (GS / 4);
+      const T* src = q + b * q_row + (int64_t)(h0 + min(column, heads - 1)) * DK + t * (GS / 4);
       constexpr int BYTES = GS / 4 * (int)sizeof(T);
       if (q_vec) {  // rows on 16-byte boundaries
 #pragma unroll
@@ -360,7 +373,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
 #pragma unroll
       for (int a = 0; a < NG; ++a)
 #pragma unroll
-        for (int i = 0; i < GS / 4; ++i) x[a][i] = g < heads ? to_f32<T>(xraw[a * (GS / 4) + i]) : 0.f;
+        for (int i = 0; i < GS / 4; ++i) x[a][i] = column < heads ? to_f32<T>(xraw[a * (GS / 4) + i]) : 0.f;
 #pragma unroll
       for (int a = 0; a < NG; ++a)
 #pragma unroll
@@ -457,6 +470,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
 #pragma unroll
     for (int a = 0; a < NG; ++a) low[a][0] = low[a][1] = 0.f;
+    const uint16_t second = t < 2 ? 0 : F16_MINUS_ONE;
     // row r of a 16-slot step is slot r, pairs swapped in the upper half of each eight: keys and values are then both
     // read from shared memory without bank conflicts at DK 64
     const int krow = g ^ ((g >> 2) & 1), vrow0 = (2 * t) ^ (t >> 1), vrow1 = (2 * t + 1) ^ (t >> 1);
@@ -666,21 +680,23 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
           low[a][0] = fmaf(s[mt][0], lo0, fmaf(s[mt][2], lo1, low[a][0]));
           low[a][1] = fmaf(s[mt][1], lo0, fmaf(s[mt][3], lo1, low[a][1]));
           float e[4] = {s[mt][0] * st0, s[mt][1] * st0, s[mt][2] * st1, s[mt][3] * st1};
-          uint32_t b0[PT], b1[PT];
+          if constexpr (PAIR) {  // columns 4 to 7: what the first term leaves
+            less_f16(e[0], e[1], pack_f16(e[0], e[1]), second);
+            less_f16(e[2], e[3], pack_f16(e[2], e[3]), second);
+          }
+          uint32_t b0[PM], b1[PM];
 #pragma unroll
-          for (int r = 0; r < PT; ++r) {
+          for (int r = 0; r < PM; ++r) {
             const uint32_t e0 = C::EXACT ? pack_bf16(e[0], e[1]) : pack_f16(e[0], e[1]);
             const uint32_t e1 = C::EXACT ? pack_bf16(e[2], e[3]) : pack_f16(e[2], e[3]);
             b0[r] = transpose8(e0);
             b1[r] = transpose8(e1);
-            if constexpr (!C::EXACT && PT > 1) {
-              const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&e0));
-              const float2 r1 = __half22float2(*reinterpret_cast<const __half2*>(&e1));
-              e[0] -= r0.x; e[1] -= r0.y;
-              e[2] -= r1.x; e[3] -= r1.y;
-            } else if constexpr (C::EXACT) {
+            if constexpr (C::EXACT) {
               e[0] -= __uint_as_float(e0 << 16); e[1] -= __uint_as_float(e0 & 0xffff0000u);
               e[2] -= __uint_as_float(e1 << 16); e[3] -= __uint_as_float(e1 & 0xffff0000u);
+            } else if constexpr (PM > 1) {
+              less_f16(e[0], e[1], e0, F16_MINUS_ONE);
+              less_f16(e[2], e[3], e1, F16_MINUS_ONE);
             }
           }
 #pragma unroll
@@ -703,7 +719,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
               const uint32_t u = mt & 1 ? ~x : x, v = mt & 1 ? ~y : y;
               const uint32_t a0 = u & 0x000f000fu, a1 = u & 0x00f000f0u, a2 = v & 0x000f000fu, a3 = v & 0x00f000f0u;
 #pragma unroll
-              for (int r = 0; r < PT; ++r) mma_f16(acc[i16], a0, a1, a2, a3, b0[r], b1[r]);
+              for (int r = 0; r < PM; ++r) mma_f16(acc[i16], a0, a1, a2, a3, b0[r], b1[r]);
             }
           }
         }
@@ -730,7 +746,8 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         const int a = i / (GS / 16);
         const float x = C::EXACT ? acc[i][c] : acc[i][c] * 16777216.f;        // f16: the codes' 2^-24
         const float y = C::EXACT ? acc[i][2 + c] : acc[i][2 + c] * 1048576.f;  // and 2^-20
-        *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(x + low[a][c], y + low[a][c]);
+        const float z = PAIR && t >= 2 ? 0.f : low[a][c];  // once per head
+        *reinterpret_cast<float2*>(row + 16 * i + 2 * g) = make_float2(x + z, y + z);
       }
       if (g == 0) {
         row[DK] = ref[c];
@@ -754,7 +771,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         const float* x = col + w * HEADS * (DK + 2);
         const float fade = x[DK] == -INFINITY ? 0.f : exp2f(x[DK] - M);
         L = fmaf(x[DK + 1], fade, L);
-        out = fmaf(x[c], fade, out);
+        out = fmaf(PAIR ? x[c] + x[4 * (DK + 2) + c] : x[c], fade, out);
       }
       if (whole) {
         o[(b * H + h0 + h) * DK + c] = from_f32<T>(p < 0 ? 0.f : out / L);
@@ -896,9 +913,15 @@ extern "C" int vb_q4_attend(const void* q, int64_t q_row, const void* k_new, int
   return VB_DISPATCH_DTYPE(dtype, T, [&]() -> int {
     auto run = [&](auto dk) -> int {
       constexpr int D = decltype(dk)::value;
-      int rc = launch_early("q4_attend", q4_attn_kernel<T, D>, ctas ? dim3(ctas) : dim3(units, B), Q4Attn<T, D>::AW * 32,
-                            Q4Attn<T, D>::SMEM, 1, st, (const T*)q, q_row, q_vec, (const T*)k_new, k_row, (const T*)v_new,
-                            v_row, pos, ring, (T*)o, part, span, ctas != 0, B, H, HKV, head_tiles, W, SLOTS, scale_log2);
+      auto attend = [&](auto pair) -> int {
+        return launch_early("q4_attend", q4_attn_kernel<T, D, decltype(pair)::value>, ctas ? dim3(ctas) : dim3(units, B),
+                            Q4Attn<T, D>::AW * 32, Q4Attn<T, D>::SMEM, 1, st, (const T*)q, q_row, q_vec, (const T*)k_new,
+                            k_row, (const T*)v_new, v_row, pos, ring, (T*)o, part, span, ctas != 0, B, H, HKV, head_tiles,
+                            W, SLOTS, scale_log2);
+      };
+      int rc;
+      if constexpr (Q4Attn<T, D>::EXACT) rc = attend(std::false_type{});
+      else rc = H / HKV <= HEADS / 2 ? attend(std::true_type{}) : attend(std::false_type{});
       if (rc || ctas == 0) return rc;
       return launch_early("q4_attend join", q4_attn_join_kernel<T, D>, dim3(HEADS, units, B), JOIN, 0, 1, st, pos,
                           (const float*)part, (const int2*)span, (T*)o, H, HKV, head_tiles);
