@@ -209,13 +209,13 @@ def q4_read(ring: Q4RingKVCache, pos: Tensor, dtype: torch.dtype = torch.bfloat1
         require_cuda("4-bit cache", ring.pos, positions=pos)
         msg = f"dtype: must be one of {SUPPORTED}, got {dtype}"
         raise ContractError(msg)
-    n = pos.shape[1]
+    n, pos = pos.shape[1], pos.contiguous()
     k = torch.empty(b, n, hkv, dk, dtype=dtype, device=device)
     v = torch.empty_like(k)
     held = torch.empty_like(pos, dtype=torch.bool, memory_format=torch.contiguous_format)
     if b and n:
         _lib.call(
-            "vb_q4_read", *_ring_ptrs(ring), pos.contiguous().data_ptr(), k.data_ptr(), v.data_ptr(), held.data_ptr(),
+            "vb_q4_read", *_ring_ptrs(ring), pos.data_ptr(), k.data_ptr(), v.data_ptr(), held.data_ptr(),
             b, n, hkv, dk, ring.window, slots, _lib.DTYPE_CODE[dtype], _lib.stream(device),
         )  # fmt: skip
     return k, v, held

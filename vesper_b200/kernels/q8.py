@@ -206,9 +206,10 @@ def dequantize_rows_q8(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.floa
         if (width > 1 and flat.stride(1) != 1) or (rows > 1 and flat.stride(0) < width):
             flat = flat.contiguous()
         pitch = flat.stride(0) if rows > 1 else width
+    scale = scale.contiguous()  # a copy is held until the launch: its memory is not to be had again before
     y = torch.empty(*q.shape, dtype=dtype, device=q.device)
     _lib.call(
-        "vb_dequantize_rows_q8", flat.data_ptr(), pitch, scale.contiguous().data_ptr(), y.data_ptr(), rows, width,
+        "vb_dequantize_rows_q8", flat.data_ptr(), pitch, scale.data_ptr(), y.data_ptr(), rows, width,
         _lib.DTYPE_CODE[dtype], _lib.stream(q.device),
     )  # fmt: skip
     return y
@@ -260,11 +261,11 @@ def linear_q8(xq: Tensor, xs: Tensor, wq: Tensor, ws: Tensor, out_dtype: torch.d
     flat = xq if xq.dim() == 2 else xq.reshape(-1, k)
     rows, ldx = _pitched(flat)
     weights, ldw = _pitched(wq)
+    xs, ws = xs.contiguous(), ws.contiguous()  # copies are held until the launch: their memory is not to be had again before
     m = xs.numel()
     y = torch.empty(m, n, dtype=out_dtype, device=device)
     _lib.call(
-        "vb_linear_q8", rows.data_ptr(), ldx, xs.contiguous().data_ptr(), weights.data_ptr(), ldw,
-        ws.contiguous().data_ptr(), y.data_ptr(), m, n, k, _lib.DTYPE_CODE[out_dtype],
-        _lib.status_word(device).data_ptr(), _lib.stream(device),
+        "vb_linear_q8", rows.data_ptr(), ldx, xs.data_ptr(), weights.data_ptr(), ldw, ws.data_ptr(), y.data_ptr(), m, n, k,
+        _lib.DTYPE_CODE[out_dtype], _lib.status_word(device).data_ptr(), _lib.stream(device),
     )  # fmt: skip
     return y if flat is xq else y.view(*xq.shape[:-1], n)
