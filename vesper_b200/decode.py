@@ -27,7 +27,7 @@ from collections.abc import Sequence
 import torch
 from torch import Tensor
 
-from vesper_b200.attention import KVCache, cache_from_ring, q4_ring_from_cache, ring_from_cache
+from vesper_b200.attention import KVCache, RingKVCache, cache_from_ring, q4_ring_from_cache, ring_from_cache
 from vesper_b200.column import ColumnState, state_tensors
 from vesper_b200.contracts import ContractError
 from vesper_b200.kernels.q4_cache import Q4RingKVCache, q4_write_
@@ -153,23 +153,26 @@ class BatchedDecoder:
             msg = "extend: at least one token is needed"
             raise ContractError(msg)
         last = self.position[:, 0]
+
+        def cache(t: int, ring: RingKVCache | Q4RingKVCache) -> KVCache:  # a pass that is not run has nothing in its ring
+            return cache_from_ring(ring, last, min(self.length, ring.window) if t < self.depth else 0, self.dtype)
+
         caches = [
-            ColumnState(h=s.h, kv=tuple(cache_from_ring(c, last, min(self.length, c.window), self.dtype) for c in s.kv),
-                        key_history=s.key_history)
+            ColumnState(h=s.h, kv=tuple(cache(t, c) for t, c in enumerate(s.kv)), key_history=s.key_history)
             for s in self.states
-        ]  # fmt: skip
+        ]
         logits, states = self._chunks(tokens, caches, self.last + 1, chunk, all_logits)
         for old, new in zip(self.states, states, strict=True):
             for dst, src in zip((*old.h, *old.key_history), (*new.h, *new.key_history), strict=True):
                 dst.copy_(src)
-            for ring, cache in zip(old.kv, new.kv, strict=True):
-                self._into_ring(ring, cache, min(length, cache.window))
+            for ring, window in zip(old.kv[: self.depth], new.kv[: self.depth], strict=True):
+                self._into_ring(ring, window, min(length, window.window))
         self.position.add_(length)
         self.length, self.last = self.length + length, self.last + length
         return logits
 
     @staticmethod
-    def _into_ring(ring: object, cache: KVCache, n: int) -> None:
+    def _into_ring(ring: RingKVCache | Q4RingKVCache, cache: KVCache, n: int) -> None:
         """The newest ``n`` entries of ``cache`` into ``ring``, in place."""
         m = cache.k.shape[1]
         k, v, pos = cache.k[:, m - n :], cache.v[:, m - n :], cache.pos[:, m - n :]
