@@ -79,3 +79,22 @@ def test_a_bf16_output_is_the_float32_result_rounded(dk: int, window: int, h: in
     o = q4_attend_(q, k, v, pos, ring)
     equal = float((o == _want(ring, q, pos).to(torch.bfloat16)).double().mean())
     assert equal >= 0.975, equal
+
+
+@pytest.mark.parametrize(("dk", "h"), [(64, 4), (128, 8)])
+def test_offsets_of_groups_that_cancel(dk: int, h: int) -> None:
+    """Keys whose groups stand far from zero, slot by slot, in amounts that the queries take from one another: parts of some
+    2000 in the scores, of which float32 keeps 2^-22 at worst, 5e-4, and the output's rounding 2e-4."""
+    b, hkv, window = 4, 1, 700
+    g = torch.Generator(device=CUDA).manual_seed(5)
+    ring = q4_ring_empty(b, hkv, dk, window, CUDA)
+    k, v = (torch.randn(b, window, hkv, dk, generator=g, device=CUDA) for _ in range(2))
+    far = 1000 * torch.randn(b, window, hkv, 1, generator=g, device=CUDA)
+    k[..., :32] += far
+    k[..., 32:64] -= far / 3
+    q4_write_(ring, k.half(), v.half(), torch.arange(window, device=CUDA).expand(b, window))
+    q, k, v, pos = _step(b, h, hkv, dk, [window] * b, 6, torch.float16)
+    q[..., :32] = (0.5 + 0.3 * q[..., :32]).bfloat16()
+    q[..., 32:64] = 3 * q[..., :32]
+    o = q4_attend_(q, k, v, pos, ring)
+    assert _rel(o, _want(ring, q, pos)) < 7e-4

@@ -62,7 +62,7 @@ struct Q4Attn {
   // rounded result, with two 0.4 %)
   static constexpr bool EXACT = sizeof(T) == 4;
   static constexpr int QT = EXACT ? 3 : 1, PT = EXACT ? 3 : 2;
-  // the sum of lo times the queries' sums as one product in bf16: four groups, two terms
+  // the sum of lo times the queries' sums as one product in bf16: four groups, three terms
   static constexpr bool LO_MMA = !EXACT && (NG == 1 || NG == 2 || NG == 4);
 };
 
@@ -415,13 +415,18 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         }
       }
       if constexpr (C::LO_MMA) {
-        // k = 2 t holds a step (times zero), k = 2 t + 1 the lo of group t, times the group's query sum in two terms
-        float mine_sum = 0.f;
+        // k = 2 t holds a step (times zero), k = 2 t + 1, 2 t + 8 and 2 t + 9 the lo of group t, times the group's query sum
+        // in three terms
+        float mine_sum = 0.f, term[3];
 #pragma unroll
         for (int a = 0; a < NG; ++a) mine_sum = t == a ? sum[a] * UNIT : mine_sum;
-        const float hi = __bfloat162float(__float2bfloat16_rn(mine_sum));
-        qlo[0] = pack_bf16(0.f, hi);
-        qlo[1] = pack_bf16(0.f, mine_sum - hi);
+#pragma unroll
+        for (int r = 0; r < 3; ++r) {
+          term[r] = __bfloat162float(__float2bfloat16_rn(mine_sum));
+          mine_sum -= term[r];
+        }
+        qlo[0] = pack_bf16(0.f, term[0]);
+        qlo[1] = pack_bf16(term[2], term[1]);
       }
       // what the sums' layout needs: heads 2 t and 2 t + 1
 #pragma unroll
@@ -529,7 +534,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         if constexpr (C::LO_MMA) {
           const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at + C::KP + r0 * C::PAR + 4 * (t % NG));
           const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + C::KP + (r0 + 8) * C::PAR + 4 * (t % NG));
-          mma_bf16_first(tot, w0, w1, w0, w1, qlo[0], qlo[1]);
+          mma_bf16_first(tot, w0, w1, __byte_perm(w0, w0, 0x3232), __byte_perm(w1, w1, 0x3232), qlo[0], qlo[1]);
         } else {
 #pragma unroll
           for (int a = 0; a < NG; ++a) {
