@@ -98,3 +98,18 @@ def test_offsets_of_groups_that_cancel(dk: int, h: int) -> None:
     q[..., 32:64] = 3 * q[..., :32]
     o = q4_attend_(q, k, v, pos, ring)
     assert _rel(o, _want(ring, q, pos)) < 7e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize(("dk", "h"), [(64, 4), (128, 8), (16, 1)])
+def test_scores_in_the_millions_and_far_beyond(dtype: torch.dtype, dk: int, h: int) -> None:
+    """One key takes all the weight, and the output is its value: off by half a step of the output's type at most, 2^-9."""
+    b, window = 3, 500
+    ring = q4_ring_empty(b, 1, dk, window, CUDA)
+    g = torch.Generator(device=CUDA).manual_seed(14)
+    k, v = (torch.randn(b, window, 1, dk, generator=g, device=CUDA) for _ in range(2))
+    q, k1, v1, pos = _step(b, h, 1, dk, [window] * b, 15, dtype)
+    for size in (2.0**8, 2.0**11, 2.0**12) if dtype == torch.float16 else (2.0**10, 2.0**14, 2.0**25, 2.0**50):
+        q4_write_(ring, (k * size).to(dtype), v.to(dtype), torch.arange(window, device=CUDA).expand(b, window))
+        o = q4_attend_((q * size).to(dtype), (k1 * size).to(dtype), v1, pos, ring)
+        assert _rel(o, _want(ring, (q * size).to(dtype), pos)) < 4e-3, size

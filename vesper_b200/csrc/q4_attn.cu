@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         }
         __syncwarp();
       }
-      // scores of slots (rows) by heads (columns), to be multiplied by f
+      // scores of slots (rows) by heads (columns), in powers of two
       float s[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -581,8 +581,10 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
           tot[2] = fmaf(s1, d[2], tot[2]);
           tot[3] = fmaf(s1, d[3], tot[3]);
         }
+        // whole scores, rounded here, so that the largest of them and the reference made of it differ by what they should
+        // however large they are
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[mt][x] = tot[x];
+        for (int x = 0; x < 4; ++x) s[mt][x] = __fmul_rn(tot[x], f[x & 1]);
       }
       if (!every) {
 #pragma unroll
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
           for (int mt = 0; mt < MT; ++mt) top[c] = fmaxf(top[c], fmaxf(s[mt][c], s[mt][2 + c]));
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
-          top[c] = fmaf(top[c], f[c], size);
+          top[c] += size;
           rise |= top[c] > ref[c] + 14.f;
         }
         if (__any_sync(0xffffffffu, rise)) {
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
               for (int a = 0; a < NG; ++a) step = fmaxf(step, q4_step(par[a]));
               const float slot_size = size_of(__float_as_uint(step));
 #pragma unroll
-              for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], fmaf(s[x / 2][x % 2 * 2 + c], f[c], slot_size));
+              for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], s[x / 2][x % 2 * 2 + c] + slot_size);
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -655,8 +657,8 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
           const float r = ref[c] == -INFINITY ? 0.f : ref[c];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            s[mt][c] = exp2_approx(fmaf(s[mt][c], f[c], -r));
-            s[mt][2 + c] = exp2_approx(fmaf(s[mt][2 + c], f[c], -r));
+            s[mt][c] = exp2_approx(s[mt][c] - r);
+            s[mt][2 + c] = exp2_approx(s[mt][2 + c] - r);
             l[c] += s[mt][c] + s[mt][2 + c];
           }
         }
