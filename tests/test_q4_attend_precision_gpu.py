@@ -113,3 +113,23 @@ def test_scores_in_the_millions_and_far_beyond(dtype: torch.dtype, dk: int, h: i
         q4_write_(ring, (k * size).to(dtype), v.to(dtype), torch.arange(window, device=CUDA).expand(b, window))
         o = q4_attend_((q * size).to(dtype), (k1 * size).to(dtype), v1, pos, ring)
         assert _rel(o, _want(ring, (q * size).to(dtype), pos)) < 4e-3, size
+
+
+@pytest.mark.parametrize("dk", [16, 64, 128])
+@pytest.mark.parametrize("h", [3, 8])
+def test_queries_at_the_upper_end_of_bf16(h: int, dk: int) -> None:
+    """Scores that stay finite: tiny keys, or queries of different sizes in one unit. A bf16 output's rounding is 2^-9."""
+    b, window = 2, 300
+    ring = q4_ring_empty(b, 1, dk, window, CUDA)
+    g = torch.Generator(device=CUDA).manual_seed(7)
+    k, v = (torch.randn(b, window, 1, dk, generator=g, device=CUDA) for _ in range(2))
+    q4_write_(ring, (k * 2.0**-95).bfloat16(), v.bfloat16(), torch.arange(window, device=CUDA).expand(b, window))
+    q, k, v, pos = _step(b, h, 1, dk, [window] * b, 8, torch.bfloat16)
+    sizes = [2.0**x for x in (95, 125, 103, 104, 105, 117, 118, 0)][:h]
+    q = q / q.abs().amax(-1, keepdim=True) * torch.tensor(sizes, device=CUDA, dtype=torch.bfloat16)[:, None]
+    k = k * 2.0**-95
+    o = q4_attend_(q, k, v, pos, ring)
+    assert bool(torch.isfinite(o).all())
+    want = _want(ring, q, pos)
+    for i in range(h):
+        assert _rel(o[:, :, i], want[:, :, i]) < 5e-3, i

@@ -63,6 +63,7 @@ struct Q4Attn {
   static constexpr bool EXACT = sizeof(T) == 4;
   static constexpr int QT = EXACT ? 3 : 1, PT = EXACT ? 3 : 2;
   // the sum of lo times the queries' sums as one product in bf16: four groups, three terms
+  static constexpr bool WIDE = std::is_same<T, __nv_bfloat16>::value;  // float32's range in 16 bits
   static constexpr bool LO_MMA = !EXACT && (NG == 1 || NG == 2 || NG == 4);
 };
 
@@ -368,6 +369,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
 
     uint32_t qb[NG][KSTEPS][QT][2], qlo[2] = {0u, 0u};
     float qs[NG][2], f[2];
+    uint32_t huge = 0;  // bit c: the scores of column 2 t + c are still to be multiplied by 2^24
     {
       float x[NG][GS / 4], top = 0.f, sum[NG];
 #pragma unroll
@@ -380,11 +382,13 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         for (int i = 0; i < GS / 4; ++i) top = fmaxf(top, fabsf(x[a][i]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // the power of two that brings the largest magnitude to [2^14, 2^15), and its inverse over the products' unit
+      // the power of two that brings the largest magnitude to [2^14, 2^15), and its inverse over the products' unit (which
+      // comes later where both would leave float32: queries from 2^104 on)
       const int e = top > 0.f ? (int)(__float_as_uint(top) >> 23) : 127;
+      const bool apart = C::WIDE && e > 230;
       const float up = __uint_as_float((uint32_t)min(268 - e, 254) << 23);
       constexpr float UNIT = C::EXACT ? 1.f : 5.9604644775390625e-8f;  // what a product's code counts: 2^-24 in f16
-      const float down = ldexpf(1.0f, (C::EXACT ? 0 : 24) - (min(268 - e, 254) - 127));
+      const float down = ldexpf(1.0f, (C::EXACT || apart ? 0 : 24) - (min(268 - e, 254) - 127));
 #pragma unroll
       for (int a = 0; a < NG; ++a) {
         sum[a] = 0.f;
@@ -433,6 +437,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
       for (int c = 0; c < 2; ++c) {
         const int from = 4 * (2 * t + c);
         f[c] = scale_log2 * __shfl_sync(0xffffffffu, down, from);
+        if constexpr (C::WIDE) huge |= (uint32_t)__shfl_sync(0xffffffffu, (int)apart, from) << c;
 #pragma unroll
         for (int a = 0; a < NG; ++a) qs[a][c] = __shfl_sync(0xffffffffu, sum[a], from) * UNIT;
       }
@@ -585,6 +590,13 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         // however large they are
 #pragma unroll
         for (int x = 0; x < 4; ++x) s[mt][x] = __fmul_rn(tot[x], f[x & 1]);
+      }
+      if (C::WIDE && huge) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (huge >> (x & 1) & 1u) s[mt][x] *= 16777216.f;
       }
       if (!every) {
 #pragma unroll
