@@ -133,3 +133,56 @@ def test_queries_at_the_upper_end_of_bf16(h: int, dk: int) -> None:
     want = _want(ring, q, pos)
     for i in range(h):
         assert _rel(o[:, :, i], want[:, :, i]) < 5e-3, i
+
+
+def _value_steps(kind: str, b: int, window: int, groups: int) -> torch.Tensor:
+    """Powers of two ``[b, slots, groups]`` for the values of a ring's slots."""
+    g = torch.Generator(device=CUDA).manual_seed(9)
+    x = torch.zeros(b, window, groups, device=CUDA)
+    if kind == "one group small":
+        x[..., 1:] = -30
+    elif kind == "one group large":
+        x[..., 0] = 45
+    elif kind == "small only later":
+        x[:, window // 2 :, 1:] = -30
+    elif kind == "small at first":
+        x[:, : window // 2, 1:] = -30
+    else:
+        x = torch.randint(-40, 41, x.shape, generator=g, device=CUDA).float()
+    return torch.exp2(x)
+
+
+@pytest.mark.parametrize("kind", ["one group small", "one group large", "small only later", "small at first", "any sizes"])
+@pytest.mark.parametrize(("dk", "h"), [(64, 4), (128, 8), (48, 3), (96, 6), (32, 5)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_groups_of_very_different_size_keep_their_own_values(dtype: torch.dtype, dk: int, h: int, kind: str) -> None:
+    """Each group of channels against its own norm, off by the output's rounding (2^-9 in bf16). f16 outputs hold no such
+    sizes, so the ring's steps are made, and the outputs compared, where f16 can tell: groups of 2^-10 and less of another."""
+    b, window, groups = 3, 1500, dk // (32 if dk % 32 == 0 else 16)
+    ring = _full(b, 1, dk, window, 10, dtype)
+    size = _value_steps(kind, b, window, groups)
+    if dtype == torch.float16:
+        size = torch.exp2(torch.log2(size) / 4)
+    ring.v_params[:, 0, :window] = (ring.v_params[:, 0, :window].float() * size[..., None]).bfloat16()
+    q, k, v, pos = _step(b, h, 1, dk, [window] * b, 11, dtype)
+    o = q4_attend_(q, k, v, pos, ring)
+    want = _want(ring, q, pos)
+    for x, y in zip(o.chunk(groups, -1), want.chunk(groups, -1), strict=True):
+        if dtype == torch.bfloat16 or float(y.abs().max()) > 2.0**-10:
+            assert _rel(x, y) < 5e-3
+
+
+def test_a_group_without_steps_before_one_of_small_steps() -> None:
+    """Constant values (no step at all) in a group's first slots, small ones later, beside a group of ordinary values."""
+    b, window, dk = 2, 1200, 64
+    g = torch.Generator(device=CUDA).manual_seed(12)
+    k, v = (torch.randn(b, window, 1, dk, generator=g, device=CUDA) for _ in range(2))
+    v[..., 32:] *= 2.0**-30
+    v[:, :700, :, 32:] = 0
+    ring = q4_write_(q4_ring_empty(b, 1, dk, window, CUDA), k.bfloat16(), v.bfloat16(), torch.arange(window, device=CUDA).expand(b, window))
+    q, k, v, pos = _step(b, 4, 1, dk, [window] * b, 13, torch.bfloat16)
+    v[..., 32:] *= 2.0**-30
+    o = q4_attend_(q, k, v, pos, ring)
+    want = _want(ring, q, pos)
+    for x, y in zip(o.chunk(2, -1), want.chunk(2, -1), strict=True):
+        assert _rel(x, y) < 5e-3

@@ -485,267 +485,285 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
     // read from shared memory without bank conflicts at DK 64
     const int krow = g ^ ((g >> 2) & 1), vrow0 = (2 * t) ^ (t >> 1), vrow1 = (2 * t + 1) ^ (t >> 1);
 
-    for (int i = 0; lo_t + warp + AW * i < hi_t; ++i) {
-      const int tile = lo_t + warp + AW * i;
-      uint8_t* at = mine + (i % C::STAGES) * C::TILE;
-      cp_async_wait<C::STAGES - 1>();
-      __syncwarp();
-      if (has_own && own_at == warp + AW * i) {  // the token takes its slot here too
-        if (tok_c < DK) {
-          const int slot = own % TS;
-          uint8_t* codes = at + (tok_value ? C::VC : 0) + slot * C::CODES;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            codes[(tok_value ? q4_value_place(DK, tok_c + 2 * j) : q4_key_place(DK, tok_c + 2 * j)) / 2] =
-                (uint8_t)(tok_codes >> (8 * j));
-          if (tok_c % GS == 0)
-            reinterpret_cast<uint32_t*>(at + (tok_value ? C::VP : C::KP))[slot * NG + tok_c / GS] = tok_params;
-        }
+    // Tiles from the i-th on. The f16 form stops at a tile in which steps lie more than 2^8 apart and the reference is to
+    // rise: from there on the products are held in three bf16 terms (X), whose range takes any steps, so that a group of large
+    // ones takes nothing from the others of its slots. Where that has not come, every group has had products of 2^-2 or
+    // more, beside which what f16 drops, 2^-25, is nothing. (Both forms in one loop cost the first 5 %.)
+    int i = 0;
+    auto walk = [&](auto exact) {
+      constexpr bool X = decltype(exact)::value;
+      constexpr int TERMS = X ? 3 : PM;
+      for (; lo_t + warp + AW * i < hi_t; ++i) {
+        const int tile = lo_t + warp + AW * i;
+        uint8_t* at = mine + (i % C::STAGES) * C::TILE;
+        cp_async_wait<C::STAGES - 1>();
         __syncwarp();
-      }
-      // which of the slots are seen
-      uint32_t seen[TS / 32];
+        if (has_own && own_at == warp + AW * i) {  // the token takes its slot here too
+          if (tok_c < DK) {
+            const int slot = own % TS;
+            uint8_t* codes = at + (tok_value ? C::VC : 0) + slot * C::CODES;
 #pragma unroll
-      for (int j = 0; j < TS / 32; ++j) {
-        const int slot = tile * TS + 32 * j + lane;
-        const int64_t kp = reinterpret_cast<const int64_t*>(at + C::POS)[32 * j + lane];
-        seen[j] = __ballot_sync(0xffffffffu, slot == own || (slot < W && kp >= 0 && (uint64_t)(p - kp) < (uint64_t)W));
-      }
-      bool every = true;
-#pragma unroll
-      for (int j = 0; j < TS / 32; ++j) every &= seen[j] == 0xffffffffu;
-      if (!every) {  // a slot that is not seen has step and lo 0, whatever it holds
-#pragma unroll
-        for (int x = 0; x < TS * NG / 32; ++x) {
-          const int slot = (32 * x + lane) / NG;
-          if (!((seen[slot >> 5] >> (slot & 31)) & 1u)) {
-            reinterpret_cast<uint32_t*>(at + C::KP)[32 * x + lane] = 0;
-            reinterpret_cast<uint32_t*>(at + C::VP)[32 * x + lane] = 0;
+            for (int j = 0; j < 4; ++j)
+              codes[(tok_value ? q4_value_place(DK, tok_c + 2 * j) : q4_key_place(DK, tok_c + 2 * j)) / 2] =
+                  (uint8_t)(tok_codes >> (8 * j));
+            if (tok_c % GS == 0)
+              reinterpret_cast<uint32_t*>(at + (tok_value ? C::VP : C::KP))[slot * NG + tok_c / GS] = tok_params;
           }
+          __syncwarp();
         }
-        __syncwarp();
-      }
-      // scores of slots (rows) by heads (columns), in powers of two
-      float s[MT][4];
+        // which of the slots are seen
+        uint32_t seen[TS / 32];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int r0 = 16 * mt + krow;
-        uint32_t c0[(DK / 8 + 3) / 4], c1[(DK / 8 + 3) / 4], p0[NG], p1[NG];
-        load_bytes<DK / 8>(at + r0 * C::CODES + t * (DK / 8), c0);
-        load_bytes<DK / 8>(at + (r0 + 8) * C::CODES + t * (DK / 8), c1);
-        load_bytes<4 * NG>(at + C::KP + r0 * C::PAR, p0);
-        load_bytes<4 * NG>(at + C::KP + (r0 + 8) * C::PAR, p1);
-        float tot[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (C::LO_MMA) {
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at + C::KP + r0 * C::PAR + 4 * (t % NG));
-          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + C::KP + (r0 + 8) * C::PAR + 4 * (t % NG));
-          mma_bf16_first(tot, w0, w1, __byte_perm(w0, w0, 0x3232), __byte_perm(w1, w1, 0x3232), qlo[0], qlo[1]);
-        } else {
-#pragma unroll
-          for (int a = 0; a < NG; ++a) {
-            // with codes as code - 7.5, lo + 7.5 step takes the place of lo
-            const float lo0 = C::EXACT ? fmaf(7.5f, q4_step(p0[a]), q4_lo(p0[a])) : q4_lo(p0[a]);
-            const float lo1 = C::EXACT ? fmaf(7.5f, q4_step(p1[a]), q4_lo(p1[a])) : q4_lo(p1[a]);
-            tot[0] = fmaf(lo0, qs[a][0], tot[0]);
-            tot[1] = fmaf(lo0, qs[a][1], tot[1]);
-            tot[2] = fmaf(lo1, qs[a][0], tot[2]);
-            tot[3] = fmaf(lo1, qs[a][1], tot[3]);
-          }
+        for (int j = 0; j < TS / 32; ++j) {
+          const int slot = tile * TS + 32 * j + lane;
+          const int64_t kp = reinterpret_cast<const int64_t*>(at + C::POS)[32 * j + lane];
+          seen[j] = __ballot_sync(0xffffffffu, slot == own || (slot < W && kp >= 0 && (uint64_t)(p - kp) < (uint64_t)W));
         }
+        bool every = true;
 #pragma unroll
-        for (int a = 0; a < NG; ++a) {
-          float d[4];
-          uint32_t w0, w1;
-          if constexpr (GS == 32) {
-            w0 = c0[a]; w1 = c1[a];
-          } else {  // four codes: the upper two in the upper half
-            w0 = (c0[a / 2] >> (16 * (a & 1))) & 0xffffu;
-            w1 = (c1[a / 2] >> (16 * (a & 1))) & 0xffffu;
-            w0 |= w0 << 8;
-            w1 |= w1 << 8;
-          }
+        for (int j = 0; j < TS / 32; ++j) every &= seen[j] == 0xffffffffu;
+        if (!every) {  // a slot that is not seen has step and lo 0, whatever it holds
 #pragma unroll
-          for (int k = 0; k < KSTEPS; ++k) {
-            const uint32_t x0 = w0 >> (8 * k), x1 = w1 >> (8 * k);
-            if constexpr (C::EXACT) {
-              const uint32_t a0 = centred(x0), a1 = centred(x1), a2 = centred(x0 >> 4), a3 = centred(x1 >> 4);
-#pragma unroll
-              for (int r = 0; r < QT; ++r) {
-                if (k == 0 && r == 0) mma_bf16_first(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
-                else mma_bf16(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
-              }
-            } else {
-              const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
-              if (k == 0) mma_f16_first(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
-              else mma_f16(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
+          for (int x = 0; x < TS * NG / 32; ++x) {
+            const int slot = (32 * x + lane) / NG;
+            if (!((seen[slot >> 5] >> (slot & 31)) & 1u)) {
+              reinterpret_cast<uint32_t*>(at + C::KP)[32 * x + lane] = 0;
+              reinterpret_cast<uint32_t*>(at + C::VP)[32 * x + lane] = 0;
             }
           }
-          const float s0 = q4_step(p0[a]), s1 = q4_step(p1[a]);
-          tot[0] = fmaf(s0, d[0], tot[0]);
-          tot[1] = fmaf(s0, d[1], tot[1]);
-          tot[2] = fmaf(s1, d[2], tot[2]);
-          tot[3] = fmaf(s1, d[3], tot[3]);
+          __syncwarp();
         }
-        // whole scores, rounded here, so that the largest of them and the reference made of it differ by what they should
-        // however large they are
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[mt][x] = __fmul_rn(tot[x], f[x & 1]);
-      }
-      if (C::WIDE && huge) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (huge >> (x & 1) & 1u) s[mt][x] *= 16777216.f;
-      }
-      if (!every) {
+        // scores of slots (rows) by heads (columns), in powers of two
+        float s[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const uint32_t bits = seen[mt >> 1] >> (16 * (mt & 1) + krow);
-          if (!(bits & 1u)) s[mt][0] = s[mt][1] = -INFINITY;
-          if (!(bits & 256u)) s[mt][2] = s[mt][3] = -INFINITY;
-        }
-      }
-      // the references, the weights and their sum
-      {
-        uint32_t big = 0;
+          const int r0 = 16 * mt + krow;
+          uint32_t c0[(DK / 8 + 3) / 4], c1[(DK / 8 + 3) / 4], p0[NG], p1[NG];
+          load_bytes<DK / 8>(at + r0 * C::CODES + t * (DK / 8), c0);
+          load_bytes<DK / 8>(at + (r0 + 8) * C::CODES + t * (DK / 8), c1);
+          load_bytes<4 * NG>(at + C::KP + r0 * C::PAR, p0);
+          load_bytes<4 * NG>(at + C::KP + (r0 + 8) * C::PAR, p1);
+          float tot[4] = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (C::LO_MMA) {
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(at + C::KP + r0 * C::PAR + 4 * (t % NG));
+            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(at + C::KP + (r0 + 8) * C::PAR + 4 * (t % NG));
+            mma_bf16_first(tot, w0, w1, __byte_perm(w0, w0, 0x3232), __byte_perm(w1, w1, 0x3232), qlo[0], qlo[1]);
+          } else {
 #pragma unroll
-        for (int x = 0; x < TS * NG / 32; ++x) big = max_bf16x2(big, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane]);
-        big = __reduce_max_sync(0xffffffffu, big << 16);  // the largest step, below 2^size
-        const float size = size_of(big);
-        float top[2];
-        bool rise = false;
+            for (int a = 0; a < NG; ++a) {
+              // with codes as code - 7.5, lo + 7.5 step takes the place of lo
+              const float lo0 = C::EXACT ? fmaf(7.5f, q4_step(p0[a]), q4_lo(p0[a])) : q4_lo(p0[a]);
+              const float lo1 = C::EXACT ? fmaf(7.5f, q4_step(p1[a]), q4_lo(p1[a])) : q4_lo(p1[a]);
+              tot[0] = fmaf(lo0, qs[a][0], tot[0]);
+              tot[1] = fmaf(lo0, qs[a][1], tot[1]);
+              tot[2] = fmaf(lo1, qs[a][0], tot[2]);
+              tot[3] = fmaf(lo1, qs[a][1], tot[3]);
+            }
+          }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          top[c] = -INFINITY;
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) top[c] = fmaxf(top[c], fmaxf(s[mt][c], s[mt][2 + c]));
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
-          top[c] += size;
-          rise |= top[c] > ref[c] + 14.f;
-        }
-        if (__any_sync(0xffffffffu, rise)) {
-          uint32_t small = 0xffffffffu;
-#pragma unroll
-          for (int x = 0; x < TS * NG / 32; ++x)
-            small = min(small, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane] << 16);
-          if ((big >> 23) - (__reduce_min_sync(0xffffffffu, small) >> 23) > 8) {
-            // steps far apart: every slot with its own, so that large values of little weight take no precision from others
-            top[0] = top[1] = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < 2 * MT; ++x) {
-              uint32_t par[NG];
-              load_bytes<4 * NG>(at + C::VP + (8 * x + krow) * C::PAR, par);
-              float step = 0.f;
-#pragma unroll
-              for (int a = 0; a < NG; ++a) step = fmaxf(step, q4_step(par[a]));
-              const float slot_size = size_of(__float_as_uint(step));
-#pragma unroll
-              for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], s[x / 2][x % 2 * 2 + c] + slot_size);
+          for (int a = 0; a < NG; ++a) {
+            float d[4];
+            uint32_t w0, w1;
+            if constexpr (GS == 32) {
+              w0 = c0[a]; w1 = c1[a];
+            } else {  // four codes: the upper two in the upper half
+              w0 = (c0[a / 2] >> (16 * (a & 1))) & 0xffffu;
+              w1 = (c1[a / 2] >> (16 * (a & 1))) & 0xffffu;
+              w0 |= w0 << 8;
+              w1 |= w1 << 8;
             }
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int k = 0; k < KSTEPS; ++k) {
+              const uint32_t x0 = w0 >> (8 * k), x1 = w1 >> (8 * k);
+              if constexpr (C::EXACT) {
+                const uint32_t a0 = centred(x0), a1 = centred(x1), a2 = centred(x0 >> 4), a3 = centred(x1 >> 4);
 #pragma unroll
-              for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
+                for (int r = 0; r < QT; ++r) {
+                  if (k == 0 && r == 0) mma_bf16_first(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+                  else mma_bf16(d, a0, a1, a2, a3, qb[a][k][r][0], qb[a][k][r][1]);
+                }
+              } else {
+                const uint32_t a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+                if (k == 0) mma_f16_first(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
+                else mma_f16(d, a0, a1, a2, a3, qb[a][k][0][0], qb[a][k][0][1]);
+              }
+            }
+            const float s0 = q4_step(p0[a]), s1 = q4_step(p1[a]);
+            tot[0] = fmaf(s0, d[0], tot[0]);
+            tot[1] = fmaf(s0, d[1], tot[1]);
+            tot[2] = fmaf(s1, d[2], tot[2]);
+            tot[3] = fmaf(s1, d[3], tot[3]);
+          }
+          // whole scores, rounded here, so that the largest of them and the reference made of it differ by what they should
+          // however large they are
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[mt][x] = __fmul_rn(tot[x], f[x & 1]);
+        }
+        if (C::WIDE && huge) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (huge >> (x & 1) & 1u) s[mt][x] *= 16777216.f;
+        }
+        if (!every) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const uint32_t bits = seen[mt >> 1] >> (16 * (mt & 1) + krow);
+            if (!(bits & 1u)) s[mt][0] = s[mt][1] = -INFINITY;
+            if (!(bits & 256u)) s[mt][2] = s[mt][3] = -INFINITY;
+          }
+        }
+        // the references, the weights and their sum
+        {
+          uint32_t big = 0;
+#pragma unroll
+          for (int x = 0; x < TS * NG / 32; ++x) big = max_bf16x2(big, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane]);
+          big = __reduce_max_sync(0xffffffffu, big << 16);  // the largest step, below 2^size
+          const float size = size_of(big);
+          float top[2];
+          bool rise = false;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            top[c] = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) top[c] = fmaxf(top[c], fmaxf(s[mt][c], s[mt][2 + c]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
+            top[c] += size;
+            rise |= top[c] > ref[c] + 14.f;
+          }
+          if (__any_sync(0xffffffffu, rise)) {
+            uint32_t small = 0xffffffffu;  // the smallest step of a slot that is seen
+#pragma unroll
+            for (int x = 0; x < TS * NG / 32; ++x) {
+              const int slot = (32 * x + lane) / NG;
+              if (every || ((seen[slot >> 5] >> (slot & 31)) & 1u))
+                small = min(small, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane] << 16);
+            }
+            if ((int)(big >> 23) - (int)(__reduce_min_sync(0xffffffffu, small) >> 23) > 8) {
+              if constexpr (!X) return;  // nothing of this tile is counted yet
+              // steps far apart: every slot with its own, so that large values of little weight take no precision from others
+              top[0] = top[1] = -INFINITY;
+#pragma unroll
+              for (int x = 0; x < 2 * MT; ++x) {
+                uint32_t par[NG];
+                load_bytes<4 * NG>(at + C::VP + (8 * x + krow) * C::PAR, par);
+                float step = 0.f;
+#pragma unroll
+                for (int a = 0; a < NG; ++a) step = fmaxf(step, q4_step(par[a]));
+                const float slot_size = size_of(__float_as_uint(step));
+#pragma unroll
+                for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], s[x / 2][x % 2 * 2 + c] + slot_size);
+              }
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float next = top[c] > ref[c] + 14.f ? top[c] - 6.f : ref[c];
+              const float fade = next == -INFINITY ? 1.f : exp2_approx(ref[c] - next);
+              ref[c] = next;
+              l[c] *= fade;
+#pragma unroll
+              for (int j = 0; j < TILES; ++j) {
+                acc[j][c] *= fade;
+                acc[j][2 + c] *= fade;
+              }
+#pragma unroll
+              for (int a = 0; a < NG; ++a) low[a][c] *= fade;
+            }
           }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float next = top[c] > ref[c] + 14.f ? top[c] - 6.f : ref[c];
-            const float fade = next == -INFINITY ? 1.f : exp2_approx(ref[c] - next);
-            ref[c] = next;
-            l[c] *= fade;
+            const float r = ref[c] == -INFINITY ? 0.f : ref[c];
 #pragma unroll
-            for (int j = 0; j < TILES; ++j) {
-              acc[j][c] *= fade;
-              acc[j][2 + c] *= fade;
+            for (int mt = 0; mt < MT; ++mt) {
+              s[mt][c] = exp2_approx(s[mt][c] - r);
+              s[mt][2 + c] = exp2_approx(s[mt][2 + c] - r);
+              l[c] += s[mt][c] + s[mt][2 + c];
+            }
+          }
+        }
+        // weights x values
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          constexpr int VB = DK / 16, VW = (VB + 3) / 4;
+          const int r0 = 16 * mt + krow;
+          uint32_t p0[NG], p1[NG], w[4][VW];
+          load_bytes<4 * NG>(at + C::VP + r0 * C::PAR, p0);
+          load_bytes<4 * NG>(at + C::VP + (r0 + 8) * C::PAR, p1);
+          const uint8_t* vc = at + C::VC + 16 * mt * C::CODES + g * VB;
+          load_bytes<VB>(vc + vrow0 * C::CODES, w[0]);
+          load_bytes<VB>(vc + vrow1 * C::CODES, w[1]);
+          load_bytes<VB>(vc + (vrow0 + 8) * C::CODES, w[2]);
+          load_bytes<VB>(vc + (vrow1 + 8) * C::CODES, w[3]);
+#pragma unroll
+          for (int a = 0; a < NG; ++a) {
+            // with codes as code - 7.5, lo + 7.5 step takes the place of lo. In f16 the odd steps of 16 slots take the codes
+            // from the other end: value = lo + 15 step - step (15 - code)
+            const float up = X ? 7.5f : mt & 1 ? 15.f : 0.f;
+            const float lo0 = fmaf(up, q4_step(p0[a]), q4_lo(p0[a])), lo1 = fmaf(up, q4_step(p1[a]), q4_lo(p1[a]));
+            const float st0 = !X && mt & 1 ? -q4_step(p0[a]) : q4_step(p0[a]);
+            const float st1 = !X && mt & 1 ? -q4_step(p1[a]) : q4_step(p1[a]);
+            low[a][0] = fmaf(s[mt][0], lo0, fmaf(s[mt][2], lo1, low[a][0]));
+            low[a][1] = fmaf(s[mt][1], lo0, fmaf(s[mt][3], lo1, low[a][1]));
+            float e[4] = {s[mt][0] * st0, s[mt][1] * st0, s[mt][2] * st1, s[mt][3] * st1};
+            if constexpr (PAIR && X) {
+              if (second) e[0] = e[1] = e[2] = e[3] = 0.f;  // columns 4 to 7 have no part in it
+            } else if constexpr (PAIR) {  // columns 4 to 7: what the first term leaves
+              less_f16(e[0], e[1], pack_f16(e[0], e[1]), second);
+              less_f16(e[2], e[3], pack_f16(e[2], e[3]), second);
+            }
+            uint32_t b0[TERMS], b1[TERMS];
+#pragma unroll
+            for (int r = 0; r < TERMS; ++r) {
+              const uint32_t e0 = X ? pack_bf16(e[0], e[1]) : pack_f16(e[0], e[1]);
+              const uint32_t e1 = X ? pack_bf16(e[2], e[3]) : pack_f16(e[2], e[3]);
+              b0[r] = transpose8(e0);
+              b1[r] = transpose8(e1);
+              if constexpr (X) {
+                e[0] -= __uint_as_float(e0 << 16); e[1] -= __uint_as_float(e0 & 0xffff0000u);
+                e[2] -= __uint_as_float(e1 << 16); e[3] -= __uint_as_float(e1 & 0xffff0000u);
+              } else if constexpr (TERMS > 1) {
+                less_f16(e[0], e[1], e0, F16_MINUS_ONE);
+                less_f16(e[2], e[3], e1, F16_MINUS_ONE);
+              }
             }
 #pragma unroll
-            for (int a = 0; a < NG; ++a) low[a][c] *= fade;
+            for (int j = 0; j < GS / 16; ++j) {
+              const int i16 = a * (GS / 16) + j;  // channels [16 i16, 16 i16 + 16): byte i16 of the lanes' parts
+              const uint32_t sel = 0x4400u + 0x1111u * (i16 % 4);
+              // that byte of two slots in the low bytes of the halves: low four bits for rows g, the others for rows g + 8
+              const uint32_t x = __byte_perm(w[0][i16 / 4], w[1][i16 / 4], sel);
+              const uint32_t y = __byte_perm(w[2][i16 / 4], w[3][i16 / 4], sel);
+              if constexpr (X) {
+                const uint32_t a0 = centred(x), a1 = centred(x >> 4), a2 = centred(y), a3 = centred(y >> 4);
+                // the matrix unit's sums are cut off, not rounded: a short one, then a rounded addition
+                float d[4];
+                mma_bf16_first(d, a0, a1, a2, a3, b0[0], b1[0]);
+#pragma unroll
+                for (int r = 1; r < TERMS; ++r) mma_bf16(d, a0, a1, a2, a3, b0[r], b1[r]);
+#pragma unroll
+                for (int e2 = 0; e2 < 4; ++e2)
+                  acc[i16][e2] = C::EXACT ? acc[i16][e2] + d[e2] : fmaf(d[e2], e2 < 2 ? 0x1p-24f : 0x1p-20f, acc[i16][e2]);
+              } else {
+                const uint32_t u = mt & 1 ? ~x : x, v = mt & 1 ? ~y : y;
+                const uint32_t a0 = u & 0x000f000fu, a1 = u & 0x00f000f0u, a2 = v & 0x000f000fu, a3 = v & 0x00f000f0u;
+#pragma unroll
+                for (int r = 0; r < TERMS; ++r) mma_f16(acc[i16], a0, a1, a2, a3, b0[r], b1[r]);
+              }
+            }
           }
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float r = ref[c] == -INFINITY ? 0.f : ref[c];
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            s[mt][c] = exp2_approx(s[mt][c] - r);
-            s[mt][2 + c] = exp2_approx(s[mt][2 + c] - r);
-            l[c] += s[mt][c] + s[mt][2 + c];
-          }
-        }
+        __syncwarp();
+        copy(i + C::STAGES);
       }
-      // weights x values
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        constexpr int VB = DK / 16, VW = (VB + 3) / 4;
-        const int r0 = 16 * mt + krow;
-        uint32_t p0[NG], p1[NG], w[4][VW];
-        load_bytes<4 * NG>(at + C::VP + r0 * C::PAR, p0);
-        load_bytes<4 * NG>(at + C::VP + (r0 + 8) * C::PAR, p1);
-        const uint8_t* vc = at + C::VC + 16 * mt * C::CODES + g * VB;
-        load_bytes<VB>(vc + vrow0 * C::CODES, w[0]);
-        load_bytes<VB>(vc + vrow1 * C::CODES, w[1]);
-        load_bytes<VB>(vc + (vrow0 + 8) * C::CODES, w[2]);
-        load_bytes<VB>(vc + (vrow1 + 8) * C::CODES, w[3]);
-#pragma unroll
-        for (int a = 0; a < NG; ++a) {
-          // with codes as code - 7.5, lo + 7.5 step takes the place of lo. In f16 the odd steps of 16 slots take the codes
-          // from the other end: value = lo + 15 step - step (15 - code)
-          const float up = C::EXACT ? 7.5f : mt & 1 ? 15.f : 0.f;
-          const float lo0 = fmaf(up, q4_step(p0[a]), q4_lo(p0[a])), lo1 = fmaf(up, q4_step(p1[a]), q4_lo(p1[a]));
-          const float st0 = !C::EXACT && mt & 1 ? -q4_step(p0[a]) : q4_step(p0[a]);
-          const float st1 = !C::EXACT && mt & 1 ? -q4_step(p1[a]) : q4_step(p1[a]);
-          low[a][0] = fmaf(s[mt][0], lo0, fmaf(s[mt][2], lo1, low[a][0]));
-          low[a][1] = fmaf(s[mt][1], lo0, fmaf(s[mt][3], lo1, low[a][1]));
-          float e[4] = {s[mt][0] * st0, s[mt][1] * st0, s[mt][2] * st1, s[mt][3] * st1};
-          if constexpr (PAIR) {  // columns 4 to 7: what the first term leaves
-            less_f16(e[0], e[1], pack_f16(e[0], e[1]), second);
-            less_f16(e[2], e[3], pack_f16(e[2], e[3]), second);
-          }
-          uint32_t b0[PM], b1[PM];
-#pragma unroll
-          for (int r = 0; r < PM; ++r) {
-            const uint32_t e0 = C::EXACT ? pack_bf16(e[0], e[1]) : pack_f16(e[0], e[1]);
-            const uint32_t e1 = C::EXACT ? pack_bf16(e[2], e[3]) : pack_f16(e[2], e[3]);
-            b0[r] = transpose8(e0);
-            b1[r] = transpose8(e1);
-            if constexpr (C::EXACT) {
-              e[0] -= __uint_as_float(e0 << 16); e[1] -= __uint_as_float(e0 & 0xffff0000u);
-              e[2] -= __uint_as_float(e1 << 16); e[3] -= __uint_as_float(e1 & 0xffff0000u);
-            } else if constexpr (PM > 1) {
-              less_f16(e[0], e[1], e0, F16_MINUS_ONE);
-              less_f16(e[2], e[3], e1, F16_MINUS_ONE);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < GS / 16; ++j) {
-            const int i16 = a * (GS / 16) + j;  // channels [16 i16, 16 i16 + 16): byte i16 of the lanes' parts
-            const uint32_t sel = 0x4400u + 0x1111u * (i16 % 4);
-            // that byte of two slots in the low bytes of the halves: low four bits for rows g, the others for rows g + 8
-            const uint32_t x = __byte_perm(w[0][i16 / 4], w[1][i16 / 4], sel);
-            const uint32_t y = __byte_perm(w[2][i16 / 4], w[3][i16 / 4], sel);
-            if constexpr (C::EXACT) {
-              const uint32_t a0 = centred(x), a1 = centred(x >> 4), a2 = centred(y), a3 = centred(y >> 4);
-              // the matrix unit's sums are cut off, not rounded: a short one, then a rounded addition
-              float d[4];
-              mma_bf16_first(d, a0, a1, a2, a3, b0[0], b1[0]);
-#pragma unroll
-              for (int r = 1; r < PT; ++r) mma_bf16(d, a0, a1, a2, a3, b0[r], b1[r]);
-#pragma unroll
-              for (int e2 = 0; e2 < 4; ++e2) acc[i16][e2] += d[e2];
-            } else {
-              const uint32_t u = mt & 1 ? ~x : x, v = mt & 1 ? ~y : y;
-              const uint32_t a0 = u & 0x000f000fu, a1 = u & 0x00f000f0u, a2 = v & 0x000f000fu, a3 = v & 0x00f000f0u;
-#pragma unroll
-              for (int r = 0; r < PM; ++r) mma_f16(acc[i16], a0, a1, a2, a3, b0[r], b1[r]);
-            }
-          }
-        }
-      }
-      __syncwarp();
-      copy(i + C::STAGES);
-    }
+    };
+    if constexpr (!C::EXACT) walk(std::false_type{});
+    walk(std::true_type{});
 
     // this warp's part: heads 2 t and 2 t + 1, channels 16 i + 2 g and 16 i + 2 g + 1
     cp_async_wait_all();  // also of copies that the position then made needless
