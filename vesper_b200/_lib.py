@@ -149,8 +149,14 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
 _STATUS: dict[torch.device, torch.Tensor] = {}
 
 
+def _indexed(device: torch.device) -> torch.device:
+    """``device`` with its index: ``cuda`` and ``cuda:0`` are one device with one status word."""
+    return device if device.index is not None else torch.device(device.type, torch.cuda.current_device())
+
+
 def status_word(device: torch.device) -> torch.Tensor:
     """The int32 the tensor-core kernels OR an error bit into (a bounded wait that gave up)."""
+    device = _indexed(device)
     word = _STATUS.get(device)
     if word is None:
         word = torch.zeros(1, dtype=torch.int32, device=device)
@@ -160,7 +166,7 @@ def status_word(device: torch.device) -> torch.Tensor:
 
 def check_status(device: torch.device) -> None:
     """Synchronise and raise if a kernel on ``device`` reported a timeout (never under capture)."""
-    word = _STATUS.get(device)
+    word = _STATUS.get(_indexed(device))
     if word is not None and int(word.item()) != 0:
         value = int(word.item())
         word.zero_()
