@@ -36,7 +36,10 @@ class TiedEmbedding(nn.Module):
         self.weight = nn.Parameter(torch.randn(vocab, d, generator=generator) / math.sqrt(d))
 
     def embed(self, tokens: Tensor) -> Tensor:
-        return F.embedding(check_ids("tokens", tokens, ("b", "n"), {}, self.vocab), self.weight)
+        ids = check_ids("tokens", tokens, ("b", "n"), {}, self.vocab)
+        if ids.is_cuda and torch.cuda.is_current_stream_capturing():
+            ids = ids.clamp(0, self.vocab - 1)  # a replay records a bad id (check_ids) and must not look it up
+        return F.embedding(ids, self.weight)
 
     def logits(self, x: Tensor) -> Tensor:
         return F.linear(x, self.weight)

@@ -22,7 +22,6 @@ from __future__ import annotations
 from collections.abc import Sequence
 
 import torch
-import torch.nn.functional as F  # noqa: N812
 from torch import Tensor
 
 from vesper_b200.column import FUSED_INPUT_DTYPES, RMS_EPS, RMS_SCALE_FLOOR, Column, ColumnState
@@ -124,7 +123,7 @@ class QuantizedVesper:
     def forward(self, token: Tensor, position: Tensor, states: Sequence[ColumnState], depth: int) -> tuple[Tensor, Tensor]:
         """The stream and the last column's output ``[b, 1, d]`` after ``depth`` dense passes over one token per row
         (``vesper_b200.decode.decode_forward``), states advanced in place."""
-        x, r = F.embedding(token, self.model.embedding.weight).float(), None
+        x, r = self.model.embedding.embed(token).float(), None
         for t in range(depth):
             if r is not None:
                 x = residual_add(x, r)
