@@ -47,3 +47,19 @@ def test_a_captured_step_records_an_id_outside_the_vocabulary(quantized: bool, b
     assert bool(torch.isfinite(logits).all())
     _lib.check_status(CUDA)
     dec.release()
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_a_refused_id_takes_no_position(quantized: bool) -> None:
+    dec, other = (_decoder(quantized, warm=9) for _ in range(2))
+    other.model.load_state_dict(dec.model.state_dict())
+    tokens = torch.tensor([[3, 7, 11, 2], [4, 9, 1, 30]], device=CUDA)
+    for x in (dec, other):
+        x.prefill(tokens[:, :2])
+    with pytest.raises(ContractError, match="every id must lie in"):
+        dec.step(torch.tensor([[1], [VOCAB]], device=CUDA))
+    torch.cuda.synchronize()
+    assert torch.equal(dec.position, other.position) and dec.length == other.length
+    for i in (2, 3):
+        want, got = (x.step(tokens[:, i : i + 1])[1] for x in (other, dec))
+        assert torch.equal(got, want)

@@ -202,8 +202,13 @@ class BatchedDecoder:
         if self.steps < self.warm:  # eager, on a side stream joined to the current one
             side = torch.cuda.Stream(self.device)
             side.wait_stream(torch.cuda.current_stream(self.device))
-            with torch.cuda.stream(side):
-                out = self._body()
+            try:
+                with torch.cuda.stream(side):
+                    out = self._body()
+            except ContractError:  # a refused token takes no position
+                torch.cuda.current_stream(self.device).wait_stream(side)
+                self.position.sub_(1)
+                raise
             torch.cuda.current_stream(self.device).wait_stream(side)
         else:
             if self.graph is None:
