@@ -1,5 +1,5 @@
 """Token ids outside the vocabulary in ``BatchedDecoder.step`` on a B200: an eager step refuses them, a captured one
-records them in the status word; neither looks them up."""
+records them in the status word; neither looks them up. What the word holds after a step is raised by the next call."""
 
 from __future__ import annotations
 
@@ -63,3 +63,35 @@ def test_a_refused_id_takes_no_position(quantized: bool) -> None:
     for i in (2, 3):
         want, got = (x.step(tokens[:, i : i + 1])[1] for x in (other, dec))
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("warm", [9, 1])
+@pytest.mark.parametrize("quantized", [False, True])
+def test_a_kernel_that_gave_up_is_raised_by_the_next_call(quantized: bool, warm: int) -> None:
+    """The bit is set by hand, as a kernel whose wait ran out sets it."""
+    dec = _decoder(quantized, warm)
+    good = torch.tensor([[1], [2]], device=CUDA)
+    calls = (lambda: dec.step(good), lambda: dec.extend(good), lambda: dec.prefill(good), dec.check)
+    for call in calls:
+        for _ in range(3):
+            dec.step(good)
+        _lib.status_word(CUDA).fill_(1)
+        dec.step(good)
+        torch.cuda.synchronize()
+        with pytest.raises(_lib.KernelError, match="status 1"):
+            call()
+        dec.prefill(good)  # raised once
+        dec.check()
+    dec.release()
+
+
+def test_a_bad_id_of_a_captured_step_is_raised_by_the_next_call() -> None:
+    dec = _decoder(True, 1)
+    good, bad = torch.tensor([[1], [2]], device=CUDA), torch.tensor([[1], [VOCAB]], device=CUDA)
+    for _ in range(3):
+        dec.step(good)
+    dec.step(bad)
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.KernelError, match="status 4"):
+        dec.step(good)
+    dec.release()

@@ -27,6 +27,7 @@ from collections.abc import Sequence
 import torch
 from torch import Tensor
 
+from vesper_b200 import _lib
 from vesper_b200.attention import KVCache, RingKVCache, cache_from_ring, q4_ring_from_cache, ring_from_cache
 from vesper_b200.column import ColumnState, state_tensors
 from vesper_b200.contracts import ContractError
@@ -96,6 +97,16 @@ class BatchedDecoder:
         self.graph: torch.cuda.CUDAGraph | None = None
         self.outputs: tuple[Tensor, Tensor] | None = None
         self.steps = 0
+        # the device's status word as the last step left it, read by the next call without waiting
+        _lib.status_word(device)
+        self._status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+
+    def check(self) -> None:
+        """Wait for the steps so far and raise ``KernelError`` if a kernel gave up or an id was out of range in one."""
+        try:
+            _lib.check_status(self.device)
+        finally:
+            self._status.zero_()
 
     def _autocast(self):
         return torch.autocast("cuda", dtype=torch.bfloat16, enabled=self.dtype == torch.bfloat16)
@@ -110,6 +121,8 @@ class BatchedDecoder:
         if b != self.b:
             msg = f"prompt of {b} rows for a decoder of {self.b}"
             raise ContractError(msg)
+        if int(self._status):
+            self.check()
         logits, states = self._chunks(tokens, self.model.init_states(b, self.dtype, self.device), 0, chunk, all_logits)
         to_ring = q4_ring_from_cache if self.quant else ring_from_cache
         rings = [ColumnState(h=s.h, kv=tuple(to_ring(c) for c in s.kv), key_history=s.key_history)
@@ -152,6 +165,8 @@ class BatchedDecoder:
         if length == 0:
             msg = "extend: at least one token is needed"
             raise ContractError(msg)
+        if int(self._status):
+            self.check()
         last = self.position[:, 0]
 
         def cache(t: int, ring: RingKVCache | Q4RingKVCache) -> KVCache:  # a pass that is not run has nothing in its ring
@@ -191,13 +206,22 @@ class BatchedDecoder:
         if self.quant is not None:
             x, r = self.quant.forward(self.token, self.position, self.states, self.depth)
             logits = self.quant.logits(x, r)[..., : self.vocab]
-            return logits.argmax(-1), logits
-        with self._autocast():
-            return decode_step(self.model, self.depth, self.vocab, self.states, self.token, self.position)
+            out = logits.argmax(-1), logits
+        else:
+            with self._autocast():
+                out = decode_step(self.model, self.depth, self.vocab, self.states, self.token, self.position)
+        self._status.copy_(_lib.status_word(self.device), non_blocking=True)
+        return out
 
     @torch.no_grad()
     def step(self, token: Tensor) -> tuple[Tensor, Tensor]:
-        """One token per row ``[b, 1]`` at the next position: ``(ids [b, 1], logits [b, 1, vocab])``."""
+        """One token per row ``[b, 1]`` at the next position: ``(ids [b, 1], logits [b, 1, vocab])``.
+
+        A kernel of a step that gave up waiting, or an id outside the vocabulary in a captured one, makes that step's
+        outputs and states wrong and raises ``KernelError`` from the first call after the step has ended (or from
+        ``check()``, which waits for it): the decoder then starts again with ``prefill``."""
+        if int(self._status):
+            self.check()
         self.token.copy_(token)
         if self.steps < self.warm:  # eager, on a side stream joined to the current one
             side = torch.cuda.Stream(self.device)
