@@ -573,6 +573,8 @@ extern "C" int vb_linear_q8(const int8_t* xq, int64_t ldx, const float* xs, cons
   VB_REQUIRE(M >= 0 && N > 0 && K > 0 && ldx >= K && ldw >= K, "linear_q8: bad shape M=%d N=%d K=%d pitches %lld, %lld",
              M, N, K, (long long)ldx, (long long)ldw);
   VB_REQUIRE(K <= 131056, "linear_q8: K=%d exceeds 131056, above which a sum may leave int32", K);
+  constexpr int MOST = INT32_MAX - 255;  // a tile more is still an int
+  VB_REQUIRE(M <= MOST && N <= MOST, "linear_q8: %d x %d outputs, of at most %d rows and columns", M, N, MOST);
   VB_REQUIRE(dtype_size(dtype) > 0, "linear_q8: unsupported dtype code %d", dtype);
   if (M == 0) return VB_OK;
   VB_REQUIRE(xq && xs && wq && ws && y && status, "linear_q8: null pointer");

@@ -30,7 +30,7 @@ from vesper_b200.contracts import ContractError, Dims, check_shape, require_cuda
 
 SUPPORTED = (torch.float32, torch.bfloat16, torch.float16)
 MAX_K = 131056  # largest inner dimension whose int8 sums stay in int32
-MAX_ROWS = 2**31 - 1  # rows of either operand
+MAX_ROWS = 2**31 - 256  # rows of either operand: with a tile more still int32
 
 
 def serving_only(what: str, *tensors: Tensor) -> None:
