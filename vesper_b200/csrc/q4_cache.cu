@@ -282,7 +282,8 @@ int check_ring(const char* what, int B, int N, int HKV, int DK, int W, int SLOTS
   VB_REQUIRE(SLOTS % Q4_TILE == 0 && SLOTS >= W, "%s: %d slots must be a multiple of %d holding the window %d", what,
              SLOTS, Q4_TILE, W);
   VB_REQUIRE(dtype_size(dtype) > 0, "%s: unsupported dtype code %d", what, dtype);
-  VB_REQUIRE(B <= 65535 && HKV <= 65535 && (int64_t)N * HKV < (int64_t(1) << 31),
+  // a CTA's tokens more are still an int
+  VB_REQUIRE(B <= 65535 && HKV <= 65535 && N <= 1 << 30 && (int64_t)N * HKV < (int64_t(1) << 31),
              "%s: %d rows of %d tokens x %d key heads exceed the grid", what, B, N, HKV);
   return VB_OK;
 }

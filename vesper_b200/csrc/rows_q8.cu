@@ -291,6 +291,7 @@ int check_rows(const char* what, int64_t rows, int width, int64_t ldq) {
   VB_REQUIRE(rows >= 0 && width > 0 && ldq >= width, "%s: bad shape rows=%lld width=%d row pitch=%lld", what,
              (long long)rows, width, (long long)ldq);
   VB_REQUIRE(rows < (int64_t(1) << 31), "%s: %lld rows exceed 2^31", what, (long long)rows);
+  VB_REQUIRE(width <= 1 << 30, "%s: rows of %d channels exceed 2^30", what, width);  // a step further is still an int
   return VB_OK;
 }
 

@@ -35,6 +35,7 @@ SUPPORTED = (torch.float32, torch.bfloat16, torch.float16)
 MAX_HEAD_DIM = 128
 SLOT_TILE = 64  # slots are allocated in whole tiles
 MAX_SLOTS = 2**31 - SLOT_TILE
+MAX_TOKENS = 2**30  # tokens of a row in one call
 
 
 def group_size(dk: int) -> int:
@@ -148,7 +149,7 @@ def _check_tokens(ring: Q4RingKVCache, k: Tensor, v: Tensor, pos: Tensor, what: 
     device = ring.pos.device
     shape = k.shape
     if not (
-        len(shape) == 4 and shape[0] == b and shape[2] == hkv and shape[3] == dk and v.shape == shape
+        len(shape) == 4 and shape[0] == b and shape[1] <= MAX_TOKENS and shape[2] == hkv and shape[3] == dk and v.shape == shape
         and pos.shape == shape[:2] and pos.dtype == torch.int64 and k.dtype in SUPPORTED and v.dtype == k.dtype
         and k.device == device and v.device == device and pos.device == device
     ):  # fmt: skip
@@ -160,6 +161,8 @@ def _check_tokens(ring: Q4RingKVCache, k: Tensor, v: Tensor, pos: Tensor, what: 
             msg = f"k, v: one dtype of {SUPPORTED}, got {k.dtype} and {v.dtype}"
             raise ContractError(msg)
         require_cuda(what, ring.pos, k=k, v=v, positions=pos)
+        msg = f"k: at most {MAX_TOKENS} tokens a row, got shape {tuple(shape)}"
+        raise ContractError(msg)
     serving_only(what, k, v)
     return b, shape[1], hkv, dk, slots
 
@@ -203,10 +206,13 @@ def q4_read(ring: Q4RingKVCache, pos: Tensor, dtype: torch.dtype = torch.bfloat1
     b, hkv, dk, slots = _check_ring(ring, "4-bit cache")
     device = ring.pos.device
     if not (
-        pos.dim() == 2 and pos.shape[0] == b and pos.dtype == torch.int64 and pos.device == device and dtype in SUPPORTED
+        pos.dim() == 2 and pos.shape[0] == b and pos.shape[1] <= MAX_TOKENS and pos.dtype == torch.int64 and pos.device == device and dtype in SUPPORTED
     ):  # fmt: skip
         check_shape("pos", pos, ("b", "n"), {"b": b}, torch.long)
         require_cuda("4-bit cache", ring.pos, positions=pos)
+        if pos.shape[1] > MAX_TOKENS:
+            msg = f"pos: at most {MAX_TOKENS} positions a row, got shape {tuple(pos.shape)}"
+            raise ContractError(msg)
         msg = f"dtype: must be one of {SUPPORTED}, got {dtype}"
         raise ContractError(msg)
     n, pos = pos.shape[1], pos.contiguous()

@@ -30,6 +30,7 @@ from vesper_b200.contracts import ContractError, Dims, check_shape, require_cuda
 
 SUPPORTED = (torch.float32, torch.bfloat16, torch.float16)
 MAX_K = 131056  # largest inner dimension whose int8 sums stay in int32
+MAX_WIDTH = 2**30  # channels of a row
 MAX_ROWS = 2**31 - 256  # rows of either operand: with a tile more still int32
 
 
@@ -40,6 +41,13 @@ def serving_only(what: str, *tensors: Tensor) -> None:
             if t.requires_grad:
                 msg = f"the {what} has no gradient: call it under torch.no_grad()"
                 raise ContractError(msg)
+
+
+def check_width(name: str, x: Tensor) -> None:
+    """Refuse rows whose width an entry point's int does not hold."""
+    if x.shape[-1] > MAX_WIDTH:
+        msg = f"{name}: rows of at most {MAX_WIDTH} channels, got shape {tuple(x.shape)}"
+        raise ContractError(msg)
 
 
 def _codes(x: Tensor) -> tuple[Tensor, Tensor, int]:
@@ -61,7 +69,7 @@ def _check_norm(x: Tensor, r: Tensor | None, weight: Tensor) -> None:
     """Accepts in one expression what is well-formed, else finds out what is not."""
     device = x.device
     if (
-        x.is_cuda and x.dtype in SUPPORTED and x.dim() >= 1 and weight.dim() == 1 and x.shape[-1] == weight.shape[0] >= 1
+        x.is_cuda and x.dtype in SUPPORTED and x.dim() >= 1 and weight.dim() == 1 and MAX_WIDTH >= x.shape[-1] == weight.shape[0] >= 1
         and weight.device == device
         and (r is None or (x.dtype == torch.float32 and r.shape == x.shape and r.dtype in SUPPORTED and r.device == device))
     ):  # fmt: skip
@@ -73,6 +81,7 @@ def _check_norm(x: Tensor, r: Tensor | None, weight: Tensor) -> None:
     if x.dim() < 1 or x.shape[-1] < 1:
         msg = f"x: expected rows of at least one channel, got shape {tuple(x.shape)}"
         raise ContractError(msg)
+    check_width("x", x)
     if weight.shape != (x.shape[-1],):
         msg = f"weight: expected shape ({x.shape[-1]},), got {tuple(weight.shape)}"
         raise ContractError(msg)
@@ -150,6 +159,7 @@ def quantize_rows_q8(x: Tensor, *, relu_square: bool = False) -> tuple[Tensor, T
     if x.dim() < 1 or x.shape[-1] < 1:
         msg = f"x: expected rows of at least one channel, got shape {tuple(x.shape)}"
         raise ContractError(msg)
+    check_width("x", x)
     width = x.shape[-1]
     if not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= width):
         x = x.contiguous()
@@ -186,7 +196,7 @@ def dequantize_rows_q8(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.floa
     """
     if not (
         q.is_cuda and scale.device == q.device and q.dtype == torch.int8 and scale.dtype == torch.float32 and q.dim() >= 1
-        and q.shape[-1] >= 1 and scale.shape == q.shape[:-1] and dtype in SUPPORTED
+        and MAX_WIDTH >= q.shape[-1] >= 1 and scale.shape == q.shape[:-1] and dtype in SUPPORTED
     ):  # fmt: skip
         require_cuda("8-bit rows", q, scale=scale)
         if q.dtype != torch.int8 or scale.dtype != torch.float32:
@@ -195,6 +205,8 @@ def dequantize_rows_q8(q: Tensor, scale: Tensor, dtype: torch.dtype = torch.floa
         if dtype not in SUPPORTED:
             msg = f"dtype: must be one of {SUPPORTED}, got {dtype}"
             raise ContractError(msg)
+        if q.dim() >= 1:
+            check_width("q", q)
         msg = f"scale: expected one per row of q {tuple(q.shape)}, got shape {tuple(scale.shape)}"
         raise ContractError(msg)
     width = q.shape[-1]
