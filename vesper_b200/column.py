@@ -117,12 +117,15 @@ def init_column_state(shape: ColumnShape, b: int, t_max: int, dtype: torch.dtype
     if t_max < 1:
         msg = f"t_max must be at least 1, got {t_max}"
         raise ValueError(msg)
+    if q4 and not ring:
+        msg = "q4 holds rings in 4 bits: it needs ring=True"
+        raise ValueError(msg)
     dk = shape.head_dim
     sdt = torch.promote_types(dtype, torch.float32)
     empty = kv_ring_empty if ring else kv_cache_empty
 
     def window() -> KVCache | RingKVCache | Q4RingKVCache:
-        if ring and q4:
+        if q4:
             return q4_ring_empty(b, shape.kv_heads, dk, shape.window, device)
         return empty(b, shape.kv_heads, dk, shape.window, dtype, device)
 
