@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from vesper_b200.column import ColumnShape, set_scan
+from vesper_b200.contracts import ContractError
 from vesper_b200.decode import BatchedDecoder
 from vesper_b200.model import Vesper
 
@@ -50,3 +51,10 @@ def test_extend_at_any_depth(depth: int, quantized: bool) -> None:
         for ring in state.kv[depth:]:
             assert not bool((ring.pos > 0).any())
     dec.release()
+
+
+def test_extending_nothing_by_nothing_is_refused_by_name() -> None:
+    model = Vesper(SHAPE, VOCAB, 1, T_MAX, 0.01, torch.Generator().manual_seed(23)).to(CUDA)
+    dec = BatchedDecoder(model, 1, VOCAB, 1)
+    with pytest.raises(ContractError, match="at least one token"):
+        dec.extend(torch.zeros(1, 0, dtype=torch.long, device=CUDA))

@@ -160,11 +160,11 @@ class BatchedDecoder:
         if b != self.b:
             msg = f"prompt of {b} rows for a decoder of {self.b}"
             raise ContractError(msg)
-        if self.length == 0:
-            return self.prefill(tokens, chunk, all_logits=all_logits)
         if length == 0:
             msg = "extend: at least one token is needed"
             raise ContractError(msg)
+        if self.length == 0:
+            return self.prefill(tokens, chunk, all_logits=all_logits)
         if int(self._status):
             self.check()
         last = self.position[:, 0]
