@@ -186,3 +186,31 @@ def test_a_group_without_steps_before_one_of_small_steps() -> None:
     want = _want(ring, q, pos)
     for x, y in zip(o.chunk(2, -1), want.chunk(2, -1), strict=True):
         assert _rel(x, y) < 5e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize(("dk", "h"), [(64, 4), (128, 8), (48, 3)])
+@pytest.mark.parametrize("kind", ["all large", "constant", "one group constant", "some tokens"])
+def test_values_at_the_upper_end_of_float32(kind: str, dk: int, h: int, dtype: torch.dtype) -> None:
+    """Outputs of up to 1e37, whole or beside small ones, constant (no step) or not: 1e-5 in float32, 2^-9 in bf16."""
+    b, window, size = 2, 900, 16 if dk % 32 else 32
+    g = torch.Generator(device=CUDA).manual_seed(16)
+    k, v = (torch.randn(b, window, 1, dk, generator=g, device=CUDA) for _ in range(2))
+    if kind == "all large":
+        v *= 1e37
+    elif kind == "constant":
+        v = torch.full_like(v, 2.0**120)
+    elif kind == "one group constant":
+        v[..., :size] = 2.0**120
+        v[..., size:] *= 1e-10
+    else:
+        v[:, 100:150] *= 1e36
+        v[:, 400] = -(2.0**122)
+    ring = q4_write_(q4_ring_empty(b, 1, dk, window, CUDA), k.to(dtype), v.to(dtype), torch.arange(window, device=CUDA).expand(b, window))
+    q, k, v, pos = _step(b, h, 1, dk, [window] * b, 17, dtype)
+    v *= 1e-10 if kind == "one group constant" else 1
+    o = q4_attend_(q, k, v, pos, ring)
+    want = _want(ring, q, pos)
+    assert bool(torch.isfinite(o).all())
+    for x, y in zip(o.split(size, -1), want.split(size, -1), strict=True):
+        assert _rel(x, y) < (1e-5 if dtype == torch.float32 else 5e-3)

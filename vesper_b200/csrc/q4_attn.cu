@@ -158,10 +158,14 @@ __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t (&w)[(BYTE
   }
 }
 
-// A power of two above a step (given as bits), as its exponent. Bounded below, where the weights' sum would leave float32;
-// and without any step the weights may be large, but not so large that a later tile's rescaling would lose them.
-__device__ __forceinline__ float size_of(uint32_t step) {
-  return step == 0 ? -40.f : (float)max((int)(step >> 23) - 126, -80);
+// What a weight may be multiplied by, as a power of two, from a largest step and a largest magnitude of lo (as bits): a power
+// above the step, between 2^-80 and 2^80, past which the weights' sum or the smaller weights would leave float32, and one by
+// which lo is at most 2^86 larger, so that no sum overflows. Without any step the weights may be large, but not so large
+// that a later tile's rescaling would lose them.
+constexpr int MOST_STEP = 80;
+__device__ __forceinline__ float size_of(uint32_t step, uint32_t lo) {
+  const int of_step = step == 0 ? -40 : min(max((int)(step >> 23) - 126, -80), MOST_STEP);
+  return (float)max(of_step, (int)(lo >> 23) - 212);
 }
 
 struct Ring {
@@ -618,9 +622,13 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         {
           uint32_t big = 0;
 #pragma unroll
-          for (int x = 0; x < TS * NG / 32; ++x) big = max_bf16x2(big, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane]);
-          big = __reduce_max_sync(0xffffffffu, big << 16);  // the largest step, below 2^size
-          const float size = size_of(big);
+          for (int x = 0; x < TS * NG / 32; ++x)
+            big = max_bf16x2(big, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane] & 0x7fff7fffu);
+          const uint32_t far = __reduce_max_sync(0xffffffffu, big & 0xffff0000u);  // the largest lo,
+          big = __reduce_max_sync(0xffffffffu, big << 16);                         // and the largest step
+          if constexpr (!X)
+            if (big >= (uint32_t)(127 + MOST_STEP) << 23) return;  // products of which f16 would overflow
+          const float size = size_of(big, far);
           float top[2];
           bool rise = false;
 #pragma unroll
@@ -649,10 +657,13 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
               for (int x = 0; x < 2 * MT; ++x) {
                 uint32_t par[NG];
                 load_bytes<4 * NG>(at + C::VP + (8 * x + krow) * C::PAR, par);
-                float step = 0.f;
+                float step = 0.f, lo = 0.f;
 #pragma unroll
-                for (int a = 0; a < NG; ++a) step = fmaxf(step, q4_step(par[a]));
-                const float slot_size = size_of(__float_as_uint(step));
+                for (int a = 0; a < NG; ++a) {
+                  step = fmaxf(step, q4_step(par[a]));
+                  lo = fmaxf(lo, fabsf(q4_lo(par[a])));
+                }
+                const float slot_size = size_of(__float_as_uint(step), __float_as_uint(lo));
 #pragma unroll
                 for (int c = 0; c < 2; ++c) top[c] = fmaxf(top[c], s[x / 2][x % 2 * 2 + c] + slot_size);
               }
