@@ -214,3 +214,20 @@ def test_values_at_the_upper_end_of_float32(kind: str, dk: int, h: int, dtype: t
     assert bool(torch.isfinite(o).all())
     for x, y in zip(o.split(size, -1), want.split(size, -1), strict=True):
         assert _rel(x, y) < (1e-5 if dtype == torch.float32 else 5e-3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dk", [64, 48, 128])
+def test_keys_at_the_upper_end_of_float32(dk: int, dtype: torch.dtype) -> None:
+    """Keys of 1e36 and queries that bring them to ordinary scores, or to finite ones of which the largest takes all."""
+    b, window = 2, 400
+    g = torch.Generator(device=CUDA).manual_seed(18)
+    k, v = (torch.randn(b, window, 1, dk, generator=g, device=CUDA) for _ in range(2))
+    ring = q4_write_(q4_ring_empty(b, 1, dk, window, CUDA), (k * 2.0**119).to(dtype), v.to(dtype), torch.arange(window, device=CUDA).expand(b, window))
+    q, k, v, pos = _step(b, 3, 1, dk, [window] * b, 19, dtype)
+    q = q * torch.tensor([2.0**-119, 2.0**-100, 1.0], device=CUDA, dtype=dtype)[:, None]
+    o = q4_attend_(q, (k.float() * 2.0**119).to(dtype), v, pos, ring)
+    want = _want(ring, q, pos)
+    assert bool(torch.isfinite(o).all())
+    for i in range(3):
+        assert _rel(o[:, :, i], want[:, :, i]) < (1e-5 if dtype == torch.float32 else 5e-3), i

@@ -386,13 +386,15 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
         for (int i = 0; i < GS / 4; ++i) top = fmaxf(top, fabsf(x[a][i]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // the power of two that brings the largest magnitude to [2^14, 2^15), and its inverse over the products' unit (which
-      // comes later where both would leave float32: queries from 2^104 on)
+      // the power of two that brings the largest magnitude to [2^14, 2^15) (in float32 to [2, 4), which leaves the keys'
+      // range to the sums), and its inverse over the products' unit (which comes later where both would leave float32:
+      // queries from 2^104 on)
       const int e = top > 0.f ? (int)(__float_as_uint(top) >> 23) : 127;
       const bool apart = C::WIDE && e > 230;
-      const float up = __uint_as_float((uint32_t)min(268 - e, 254) << 23);
+      const int up_e = min((C::EXACT ? 255 : 268) - e, 254);
+      const float up = __uint_as_float((uint32_t)up_e << 23);
       constexpr float UNIT = C::EXACT ? 1.f : 5.9604644775390625e-8f;  // what a product's code counts: 2^-24 in f16
-      const float down = ldexpf(1.0f, (C::EXACT || apart ? 0 : 24) - (min(268 - e, 254) - 127));
+      const float down = ldexpf(1.0f, (C::EXACT || apart ? 0 : 24) - (up_e - 127));
 #pragma unroll
       for (int a = 0; a < NG; ++a) {
         sum[a] = 0.f;
