@@ -64,7 +64,7 @@ __device__ __forceinline__ void q4_params(float low, float high, float& step, fl
   const float q = __fmul_rn(span, FIFTEENTH);
   const float exact = __fmaf_rn(__fmaf_rn(-q, 15.0f, span), FIFTEENTH, q);
   step = span < Q4_FLAT ? 0.f : __uint_as_float((__float_as_uint(exact) + 0xffffu) & 0xffff0000u);
-  if (!(fabsf(lo) <= 3.4e38f && span <= 3.4e38f)) lo = step = __uint_as_float(0x7fc00000u);  // also for a NaN
+  if (!(fabsf(lo) < INFINITY && span < INFINITY)) lo = step = __uint_as_float(0x7fc00000u);  // also for a NaN
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(step));
   inverse = step > 0.f ? __fmaf_rn(__fmaf_rn(-step, r, 1.0f), r, r) : 0.f;
