@@ -231,3 +231,25 @@ def test_keys_at_the_upper_end_of_float32(dk: int, dtype: torch.dtype) -> None:
     assert bool(torch.isfinite(o).all())
     for i in range(3):
         assert _rel(o[:, :, i], want[:, :, i]) < (1e-5 if dtype == torch.float32 else 5e-3), i
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("order", ["ordinary first", "far below first", "in turn"])
+@pytest.mark.parametrize(("dk", "h"), [(64, 4), (128, 7)])
+def test_ordinary_scores_beside_scores_in_the_millions(dk: int, h: int, order: str, dtype: torch.dtype) -> None:
+    """Tiles of ordinary keys and of keys 2^30 times as large: of those the one that scores most takes all, or, where they all
+    score far below, the ordinary ones share it. Off by the output's rounding, 2^-9, in float32 by 1e-5."""
+    b, window = 2, 1500
+    g = torch.Generator(device=CUDA).manual_seed(71)
+    k, v = (torch.randn(b, window, 1, dk, generator=g, device=CUDA) for _ in range(2))
+    q, k1, v1, pos = _step(b, h, 1, dk, [window] * b, 72, dtype)
+    if order == "ordinary first":
+        k[:, window // 2 :] *= 2.0**30
+    elif order == "far below first":
+        k[:, : window // 2] = -(2.0**30) * q[:, :, :1].float().mean(2, keepdim=True)
+        q = q[:, :, :1].expand(b, 1, h, dk).contiguous()
+    else:
+        k[:, ::3] *= 2.0**30
+    ring = q4_write_(q4_ring_empty(b, 1, dk, window, CUDA), k.to(dtype), v.to(dtype), torch.arange(window, device=CUDA).expand(b, window))
+    o = q4_attend_(q, k1, v1, pos, ring)
+    assert _rel(o, _want(ring, q, pos)) < (1e-5 if dtype == torch.float32 else 4e-3)

@@ -26,13 +26,14 @@
 // a second kernel, in a fixed order. A slot that is not seen has score -inf and its step and lo are read as zeros,
 // whatever it holds.
 //
-// Measured (bf16, device): 8 rows of 6249 to 49999 positions, 32 query and 8 key heads of 128, 62 us (290 MB, 4.7
-// TB/s, 71 % of a plain copy's rate); 8 x 32768 70 us (4.8 TB/s, 74 %). What keeps it from the copy's rate is
-// latency: eight warps an SM (238 registers each at DK 128) issue in half of the cycles, and the last tiles of a unit, the
+// Measured (bf16, device): 8 rows of 6249 to 49999 positions, 32 query and 8 key heads of 128, 67 us (290 MB, 4.3
+// TB/s, 66 % of a plain copy's rate); 8 x 32768 76 us (4.45 TB/s, 68 %). What keeps it from the copy's rate is
+// latency: eight warps an SM (255 registers each at DK 128) issue in half of the cycles, and the last tiles of a unit, the
 // joining of its warps and the next unit's first tiles follow one another. At DK 64, eight query heads to two key heads,
-// 64 x 8192 take 30.7 us (88 MB, 44 %): half the bytes for each instruction. 64 rows of 512 positions take 5.4 us, the
+// 64 x 8192 take 33 us (88 MB, 41 %): half the bytes for each instruction. 64 rows of 512 positions take 5.7 us, the
 // latency of position, tiles, two products and the joining. One float32 row of 100003 positions at DK 64,
-// three products for one, takes 21 us.
+// three products for one, takes 21.5 us. Of the first two figures some 8 % buy what 16-bit outputs keep: the second term of
+// the products 4 us of the 76, sums and ranges 2.
 #include <cmath>
 #include <type_traits>
 
@@ -260,7 +261,7 @@ struct Share {
 // the last CTA of a unit. Else a CTA per unit and row.
 // PAIR: at most four heads to a key head. Columns 4 to 7 of the products then repeat the heads of columns 0 to 3, bit for bit,
 // and take the second f16 term of the weights' products, so that two terms cost no second product (8 x 32768 positions, 32 /
-// 8 heads of 128: 75 us, with two products 82; a single term 72).
+// 8 heads of 128, when this was chosen: 75 us, with two products 82, a single term 71).
 template <typename T, int DK, bool PAIR>
 __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
     q4_attn_kernel(const T* __restrict__ q, int64_t q_row, int q_vec, const T* __restrict__ k_new, int64_t k_row,
@@ -491,10 +492,12 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
     // read from shared memory without bank conflicts at DK 64
     const int krow = g ^ ((g >> 2) & 1), vrow0 = (2 * t) ^ (t >> 1), vrow1 = (2 * t + 1) ^ (t >> 1);
 
-    // Tiles from the i-th on. The f16 form stops at a tile in which steps lie more than 2^8 apart and the reference is to
-    // rise: from there on the products are held in three bf16 terms (X), whose range takes any steps, so that a group of large
-    // ones takes nothing from the others of its slots. Where that has not come, every group has had products of 2^-2 or
-    // more, beside which what f16 drops, 2^-25, is nothing. (Both forms in one loop cost the first 5 %.)
+    // Tiles from the i-th on, in f16 as far as it goes. That form stops at a tile where the reference is to rise and steps lie
+    // more than 2^8 apart: from there on the products are held in three bf16 terms (X), whose range takes any steps, so that a
+    // group of large ones takes nothing from the others of its slots. Where that has not come, every group has had products of
+    // 2^-2 or more, beside which what f16 drops, 2^-25, is nothing. It stops too before a reference of 2^20, beside which the
+    // rounding of the reference itself would begin to count, and before steps of 2^80. (Both forms in one loop cost 5 %,
+    // whole scores in it 3 %.)
     int i = 0;
     auto walk = [&](auto exact) {
       constexpr bool X = decltype(exact)::value;
@@ -539,7 +542,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
           }
           __syncwarp();
         }
-        // scores of slots (rows) by heads (columns), in powers of two
+        // scores of slots (rows) by heads (columns)
         float s[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -600,10 +603,10 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
             tot[2] = fmaf(s1, d[2], tot[2]);
             tot[3] = fmaf(s1, d[3], tot[3]);
           }
-          // whole scores, rounded here, so that the largest of them and the reference made of it differ by what they should
-          // however large they are
+          // X: whole scores, rounded here, so that the largest of them and the reference made of it differ by what they
+          // should however large they are; else still to be multiplied by f
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[mt][x] = __fmul_rn(tot[x], f[x & 1]);
+          for (int x = 0; x < 4; ++x) s[mt][x] = X ? __fmul_rn(tot[x], f[x & 1]) : tot[x];
         }
         if (C::WIDE && huge) {
 #pragma unroll
@@ -640,7 +643,7 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
             for (int mt = 0; mt < MT; ++mt) top[c] = fmaxf(top[c], fmaxf(s[mt][c], s[mt][2 + c]));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
-            top[c] += size;
+            top[c] = fmaf(top[c], X ? 1.f : f[c], size);
             rise |= top[c] > ref[c] + 14.f;
           }
           if (__any_sync(0xffffffffu, rise)) {
@@ -651,8 +654,11 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
               if (every || ((seen[slot >> 5] >> (slot & 31)) & 1u))
                 small = min(small, reinterpret_cast<const uint32_t*>(at + C::VP)[32 * x + lane] << 16);
             }
-            if ((int)(big >> 23) - (int)(__reduce_min_sync(0xffffffffu, small) >> 23) > 8) {
-              if constexpr (!X) return;  // nothing of this tile is counted yet
+            const bool apart = (int)(big >> 23) - (int)(__reduce_min_sync(0xffffffffu, small) >> 23) > 8;
+            if constexpr (!X) {  // nothing of this tile is counted yet
+              const bool steep = (fabsf(top[0]) >= 0x1p20f && top[0] != -INFINITY) || (fabsf(top[1]) >= 0x1p20f && top[1] != -INFINITY);
+              if (__any_sync(0xffffffffu, apart || steep)) return;
+            } else if (apart) {
               // steps far apart: every slot with its own, so that large values of little weight take no precision from others
               top[0] = top[1] = -INFINITY;
 #pragma unroll
@@ -694,8 +700,8 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
             const float r = ref[c] == -INFINITY ? 0.f : ref[c];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              s[mt][c] = exp2_approx(s[mt][c] - r);
-              s[mt][2 + c] = exp2_approx(s[mt][2 + c] - r);
+              s[mt][c] = exp2_approx(X ? s[mt][c] - r : fmaf(s[mt][c], f[c], -r));
+              s[mt][2 + c] = exp2_approx(X ? s[mt][2 + c] - r : fmaf(s[mt][2 + c], f[c], -r));
               l[c] += s[mt][c] + s[mt][2 + c];
             }
           }
