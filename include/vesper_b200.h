@@ -381,6 +381,7 @@ VB_API int vb_nll_row_grad(void *logits, int64_t stride, const int64_t *targets,
  * code = rint(y * 127 / max|y|). A row of magnitude below 1e-35 has scale 0 and codes 0; a row that
  * holds a value that is not finite has scale NaN and codes 0 (it stands for NaN everywhere).
  * q: int8 rows `ldq` bytes apart (ldq >= width; the bytes between width and ldq are not written).
+ * Fewer than 2^31 rows of at most 2^30 channels.
  *
  * vb_rms_norm_q8: y is the RMSNorm of x (vb_rms_norm_fwd's arithmetic, vesper/column.py:159-188), or,
  * with r, of sum = x + r (x, sum float32; r float32, bf16 or f16, r and sum both given or both NULL).
@@ -395,7 +396,7 @@ VB_API int vb_dequantize_rows_q8(const int8_t *q, int64_t ldq, const float *scal
                                  int64_t rows, int width, int dtype, void *stream);
 
 /* The quantised linear layer: y [M, N] of `dtype` (dense) = (sum_k xq[m,k] wq[n,k]) xs[m] ws[n], the
- * sum exact in int32 (K <= 131056), scaled in float32 and rounded once. xq [M, K] and wq [N, K] int8,
+ * sum exact in int32 (K <= 131056; M and N <= 2^31 - 256), scaled in float32 and rounded once. xq [M, K] and wq [N, K] int8,
  * rows ldx and ldw bytes apart, 16-byte aligned, ldx and ldw multiples of 16; xs [M], ws [N] float32.
  * `status`: an int32 on the device into which a kernel ORs 1 if a bounded wait gave up. Takes the
  * place of the F.linear of vesper/column.py:236-253 and vesper/ffn.py:44-56 in quantised decoding. */
@@ -415,7 +416,7 @@ VB_API int vb_linear_q8(const int8_t *xq, int64_t ldx, const float *xs, const in
  *
  * vb_q4_write: tokens k, v [B, N, HKV, DK] (batch and token strides in elements) at pos [B, N] int64,
  * consecutive along a row; a negative position (padding) is not written, and of tokens that share a
- * slot (N > W) the last is kept. vb_q4_read: the values held at pos [B, N], zeros and held = 0 where
+ * slot (N > W) the last is kept (N <= 2^30 here and in vb_q4_read). vb_q4_read: the values held at pos [B, N], zeros and held = 0 where
  * the ring does not hold that position. vb_q4_attend: one token per row, q [B, H, DK], k_new, v_new
  * [B, HKV, DK] (row strides in elements), pos [B]: the token is written and attends the slots with
  * p - W < pos <= p, itself included, as the ring holds them (scale 1/sqrt(DK), head h reading key

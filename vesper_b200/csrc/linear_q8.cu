@@ -14,8 +14,9 @@
 //   on CTA pairs (cta_group::2), each CTA copying half of either operand (32 KB per 128 bytes of K, against 48 KB for
 //   a single CTA's 128 x 256). Accumulators are double-buffered in TMEM, so that the storing warps' loads,
 //   scaling and TMA stores run under the next tile's products. 8192 x 4096 x 8192 in 184 us, 2.98 POP/s, the tensor
-//   pipe active 75 % of the time (before the pairs 236 us, before the doubled accumulators 271); 777 x 1040 x 2001,
-//   91 tiles of nine blocks of K on 148 SMs, in 8.4 us: the latency of one tile.
+//   pipe active 75 % of the time (before the pairs 236 us, before the doubled accumulators 271). Longer K adds 43 ns a
+//   byte of it, 3.14 POP/s, so some 15 us are the kernel's start, its last tiles and their stores; 777 x 1040 x 2001,
+//   112 tiles of nine blocks of K on 148 SMs, in 8.8 us: the latency of one tile.
 #include <cmath>
 
 #include "launch.cuh"

@@ -220,7 +220,7 @@ __device__ __forceinline__ void find_row(const int64_t* pos, int B, int units, i
 
 // All rows' and units' costs, and how many of a launch's CTAs share them: as many as have a tile for each of their warps,
 // but one for each unit that sees something if that is more. An opening counts 16 tiles where a CTA has over 32 (8
-// streams of 6249 to 49999 positions, 8 key heads of 128: 61 us, with none 67, with 40 63), none where it has fewer.
+// streams of 6249 to 49999 positions, 8 key heads of 128, when this was chosen: 61 us, with none 67, with 40 63), none where it has fewer.
 template <int TS, int AW>
 __device__ __forceinline__ int64_t all_costs(const int64_t* pos, int B, int units, int W, int& ctas, int& opening) {
   int64_t sum = 0;

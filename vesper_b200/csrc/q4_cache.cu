@@ -4,9 +4,10 @@
 // extremes from a thread's registers and its neighbour's, and the codes by way of shared memory, where they find their
 // places a byte or a word at a time and leave or arrive in 8-byte pieces of consecutive slots. HBM bound: 2 bytes in and
 // 0.625 out per bf16 channel, or the reverse. 4 x 32701 tokens, 8 heads of 128, are written in 144 us (4.9 TB/s, 75 % of
-// a plain copy's rate; instructions issue in 80 % of the cycles) and read back in 148 us (4.75 TB/s, 73 %: 3.6
-// TB/s of stores, as much as filling memory reaches). float32 tokens, with twice the bytes for each, are written at 6.1
-// TB/s (93 %). 64 x 2048 tokens into a window of 512, one head of 64: 6.3 and 6.0 us.
+// a plain copy's rate; instructions issue in 80 % of the cycles) and read back in 148 us (4.75 TB/s, 73 %; instructions
+// issue in 72 % of the cycles, and memory would take more: float32, with half the codes for its bytes, is stored at 4.9 TB/s
+// where this stores 3.6). float32 tokens, with twice the bytes for each, are written at 6.1
+// TB/s (93 %). 64 x 2048 tokens into a window of 512, two heads of 64: 6.3 and 5.9 us.
 #include <type_traits>
 
 #include "launch.cuh"

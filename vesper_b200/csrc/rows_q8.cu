@@ -14,7 +14,8 @@
 // HBM bound: 4 + 2 + 4 + 1 bytes per channel for a float32 stream with a bf16 addend. Measured, in turn with other
 // inputs: 32768 x 512 in 29.7 us (6.2 TB/s, 95 % of a plain copy's rate), 8192 x 5000 in 72 us (6.2 TB/s), 16384 x 2048
 // in 56.5 us (6.5 TB/s); a kernel that reads the row anew for every step takes 108, 113 and 84. 64 x 512 takes 1.8 us,
-// the latency of one load, two reductions and a launch.
+// the latency of one load, two reductions and a launch. Plain rows: 64 x 512 of bf16 1.5 us, 64 x 1536 with the squared ReLU
+// 1.7, 32768 x 512 10.1 (5.0 TB/s), 32768 x 1536 with the squared ReLU 37 (4.0 TB/s), 8192 x 4096 of float32 25 (6.7 TB/s).
 #include <type_traits>
 
 #include "launch.cuh"
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(NT* RPC) rows_q8_kernel(const TX* __restrict__
 }
 
 // Any width, any alignment: a CTA per row, the row read once per step, the second and third time from L2 (8192 x 4096:
-// 82 us, in registers 56).
+// 82 us, in registers 56; 8192 x 9000, wider than registers hold, 239 us for the 124 of its bytes).
 template <typename TX, typename TR, int MODE>
 __global__ void __launch_bounds__(256) rows_q8_any_kernel(const TX* __restrict__ x, int64_t ldx,
                                                           const TR* __restrict__ r, const float* __restrict__ w,
