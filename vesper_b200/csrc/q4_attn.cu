@@ -59,7 +59,8 @@ struct Q4Attn {
   static constexpr int AW = 8, STAGES = 2, CTAS = ctas_per_sm(DK);  // warps per CTA, tiles in flight per warp
   static constexpr int SMEM = AW * STAGES * TILE;
   // float32 throughout: queries and the weights' products in three bf16 terms, codes as code - 7.5. Else queries in one
-  // f16 term, which a 16-bit query is, and the products in two (with one, 17 % of a bf16 output's numbers are not the
+  // f16 term, which a 16-bit query is (but for bf16 channels 2^28 below their head's largest: they lose their last bits, 2^-36
+  // of the largest), and the products in two (with one, 17 % of a bf16 output's numbers are not the
   // rounded result, with two 0.4 %)
   static constexpr bool EXACT = sizeof(T) == 4;
   static constexpr int QT = EXACT ? 3 : 1, PT = EXACT ? 3 : 2;
@@ -220,7 +221,8 @@ __device__ __forceinline__ void find_row(const int64_t* pos, int B, int units, i
 
 // All rows' and units' costs, and how many of a launch's CTAs share them: as many as have a tile for each of their warps,
 // but one for each unit that sees something if that is more. An opening counts 16 tiles where a CTA has over 32 (8
-// streams of 6249 to 49999 positions, 8 key heads of 128, when this was chosen: 61 us, with none 67, with 40 63), none where it has fewer.
+// streams of 6249 to 49999 positions, 8 key heads of 128, when this was chosen: 61 us, with none 67, with 40 63), none
+// where it has fewer.
 template <int TS, int AW>
 __device__ __forceinline__ int64_t all_costs(const int64_t* pos, int B, int units, int W, int& ctas, int& opening) {
   int64_t sum = 0;
@@ -656,7 +658,8 @@ __global__ void __launch_bounds__(Q4Attn<T, DK>::AW * 32, (Q4Attn<T, DK>::CTAS))
             }
             const bool apart = (int)(big >> 23) - (int)(__reduce_min_sync(0xffffffffu, small) >> 23) > 8;
             if constexpr (!X) {  // nothing of this tile is counted yet
-              const bool steep = (fabsf(top[0]) >= 0x1p20f && top[0] != -INFINITY) || (fabsf(top[1]) >= 0x1p20f && top[1] != -INFINITY);
+              const bool steep = (fabsf(top[0]) >= 0x1p20f && top[0] != -INFINITY) ||
+                                 (fabsf(top[1]) >= 0x1p20f && top[1] != -INFINITY);
               if (__any_sync(0xffffffffu, apart || steep)) return;
             } else if (apart) {
               // steps far apart: every slot with its own, so that large values of little weight take no precision from others

@@ -206,7 +206,8 @@ def q4_read(ring: Q4RingKVCache, pos: Tensor, dtype: torch.dtype = torch.bfloat1
     b, hkv, dk, slots = _check_ring(ring, "4-bit cache")
     device = ring.pos.device
     if not (
-        pos.dim() == 2 and pos.shape[0] == b and pos.shape[1] <= MAX_TOKENS and pos.dtype == torch.int64 and pos.device == device and dtype in SUPPORTED
+        pos.dim() == 2 and pos.shape[0] == b and pos.shape[1] <= MAX_TOKENS and pos.dtype == torch.int64
+        and pos.device == device and dtype in SUPPORTED
     ):  # fmt: skip
         check_shape("pos", pos, ("b", "n"), {"b": b}, torch.long)
         require_cuda("4-bit cache", ring.pos, positions=pos)
